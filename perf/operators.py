@@ -13,7 +13,7 @@ import torch
 
 own = False
 
-E_MIN, E_MAX, CODE_MAX = -100, 119, 448.0
+E_MIN, E_MAX, CODE_MAX = -40, 119, 448.0
 DEV = "cuda"
 
 
