@@ -25,7 +25,8 @@ NVCC_FLAGS = [
 ]
 
 # sources that keep the accurate forms of exp, division and square root
-ACCURATE = {"latent.cu", "memory.cu", "memory_chunk.cu", "grouped.cu", "moe.cu", "depth.cu", "delta.cu", "delta_chunk.cu"}
+ACCURATE = {"latent.cu", "memory.cu", "memory_chunk.cu", "grouped.cu", "moe.cu", "depth.cu", "delta.cu", "delta_chunk.cu",
+            "kv8.cu", "kv8_attention.cu", "sample.cu"}
 
 
 def flags_for(src: str) -> list:

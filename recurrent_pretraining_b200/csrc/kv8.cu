@@ -1,0 +1,290 @@
+// Writing and reading the 8-bit key / value cache (kv8.cuh):
+//   * kv8_append       : n tokens per sequence, any start, one CTA per (sequence, head, touched block, keys or values)
+//   * kv8_rope_append  : the one new token of a decode step from its packed projection: bias, rotation, q out, k and v encoded
+//   * kv8_decode       : codes back to bf16 rows [B, L, Hkv, D] (exact), as the prompt attention reads them
+//   * kv8_tiles        : tile table of the prompt attention, from the lengths on the device
+//
+// A block that is begun takes the exponent of its new tokens, so what lay in the cache before does not matter and freed rows need
+// no clearing.  A block that goes on keeps the larger of both exponents; when the new tokens' is larger, what it holds in front of
+// them is encoded again by the CTA (or lane group) that writes them.  Writing the same tokens to the same place again
+// changes nothing: exponents only grow.  Nothing behind the new tokens is touched.
+#include "kv8.cuh"
+
+namespace b200 {
+
+struct Kv8Cache {
+  uint8_t *k, *v;                    // codes
+  int8_t *ke, *ve;                   // exponents
+  long long sb, sh, eb, eh;          // batch and head pitch of codes and exponents (elements)
+  int B, Hkv, cap, D, log2_block;
+};
+
+// grid (2 x most touched blocks, Hkv, B), 128 threads.  The block's new tokens stay in registers (NV vectors of eight values per
+// thread) between the maximum and the encoding: one pass over the input.
+template <int NV>
+__global__ void __launch_bounds__(128)
+kv8_append_kernel(const Kv8Cache c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long k_sb,
+                  long long k_sn, long long k_sh, long long v_sb, long long v_sn, long long v_sh, const int* __restrict__ start_,
+                  const int* __restrict__ counts, int n, int* err) {
+  pdl_trigger();
+  pdl_wait();
+  const int which = blockIdx.x & 1, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int start = start_[b], cnt = counts ? counts[b] : n;
+  if (start < 0 || cnt < 0 || cnt > n || start > c.cap - cnt) {     // the sequence does not fit: nothing of it is written
+    if (tid == 0 && err) atomicCAS(err, 0, ERR_BAD_INDEX);
+    return;
+  }
+  const int block = (start >> c.log2_block) + (blockIdx.x >> 1), p0 = block << c.log2_block;
+  const int lo = max(start, p0), hi = min(start + cnt, p0 + (1 << c.log2_block));
+  if (lo >= hi) return;
+  const long long sn = which ? v_sn : k_sn;
+  const __nv_bfloat16* src = (which ? v + b * v_sb + h * v_sh : k + b * k_sb + h * k_sh) + (lo - start) * sn;
+  uint8_t* dst = (which ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(p0) * c.D;
+  int8_t* ep = (which ? c.ve : c.ke) + b * c.eb + h * c.eh + block;
+  const int vpr = c.D >> 3, nvec = (hi - lo) * vpr;
+  uint4 x[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int idx = tid + 128 * i;
+    x[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (idx < nvec) x[i] = __ldg(reinterpret_cast<const uint4*>(src + (idx / vpr) * sn) + idx % vpr);
+  }
+  const bool fresh = lo == p0;
+  const int old = fresh ? KV8_EMIN : *ep;
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_bf16x2(w[j]);
+      amax = fmaxf(amax, fmaxf(kv8_mag(f.x), kv8_mag(f.y)));
+    }
+  }
+  __shared__ float red[4];
+  amax = warp_max(amax);
+  if ((tid & 31) == 0) red[tid >> 5] = amax;
+  __syncthreads();                                                  // every thread has read the old exponent, too
+  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int e = max(kv8_exponent(amax), old);
+  const float inv = pow2i(-e);
+  if (tid == 0) *ep = static_cast<int8_t>(e);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int idx = tid + 128 * i;
+    if (idx < nvec) {
+      const float2 f0 = unpack_bf16x2(x[i].x), f1 = unpack_bf16x2(x[i].y), f2 = unpack_bf16x2(x[i].z), f3 = unpack_bf16x2(x[i].w);
+      *reinterpret_cast<uint2*>(dst + static_cast<size_t>(lo - p0) * c.D + 8 * static_cast<size_t>(idx)) =
+          make_uint2(kv8_encode4(f0.x, f0.y, f1.x, f1.y, inv), kv8_encode4(f2.x, f2.y, f3.x, f3.y, inv));
+    }
+  }
+  if (!fresh && e > old) {
+    const float f = pow2i(old - e);
+    for (int idx = tid; idx < (lo - p0) * vpr; idx += 128) {
+      uint2* w = reinterpret_cast<uint2*>(dst) + idx;
+      *w = make_uint2(kv8_recode4(w->x, f), kv8_recode4(w->y, f));
+    }
+  }
+}
+
+// One group of 16 lanes per (sequence, head of q, k or v), eight channels per lane.  F32_IN: the projection is an fp32 accumulator,
+// handed back zeroed when `clear` is set.  Values reach the codes from fp32 directly (one rounding); q is rounded once, to bf16.
+template <bool F32_IN>
+__global__ void __launch_bounds__(256)
+kv8_rope_append_kernel(const Kv8Cache c, void* __restrict__ qkv, long long ld, const float* __restrict__ bias,
+                       const float* __restrict__ cosT, const float* __restrict__ sinT, const int* __restrict__ pos,
+                       __nv_bfloat16* __restrict__ q_out, int H, int clear, int* err) {
+  pdl_trigger();
+  const int heads = H + 2 * c.Hkv;
+  const int unit = blockIdx.x * 16 + (threadIdx.x >> 4), j = threadIdx.x & 15;
+  const bool live = unit < c.B * heads && 8 * j < c.D;
+  const int b = live ? unit / heads : 0, hh = live ? unit - b * heads : 0;
+  const bool rotated = hh < H + c.Hkv;
+  float add[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) add[i] = 0.f;
+  if (live && rotated && bias) {                                    // does not depend on the predecessor
+#pragma unroll
+    for (int i = 0; i < 8; ++i) add[i] = bias[hh * c.D + 8 * j + i];
+  }
+  pdl_wait();
+  const int p = live ? pos[b] : 0;
+  const bool ok = live && p >= 0 && p < c.cap;
+  if (live && !ok && err) atomicCAS(err, 0, ERR_BAD_INDEX);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (live) {
+    if constexpr (F32_IN) {
+      float4* src = reinterpret_cast<float4*>(static_cast<float*>(qkv) + b * ld + hh * c.D + 8 * j);
+      const float4 a = src[0], d = src[1];
+      if (clear) src[0] = src[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = d.x; x[5] = d.y; x[6] = d.z; x[7] = d.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(qkv) + b * ld + hh * c.D + 8 * j);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_bf16x2(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
+  if (ok && rotated) {
+    const float4 cs = *reinterpret_cast<const float4*>(cosT + static_cast<size_t>(p) * (c.D >> 1) + 4 * j);
+    const float4 sn = *reinterpret_cast<const float4*>(sinT + static_cast<size_t>(p) * (c.D >> 1) + 4 * j);
+    const float cw[4] = {cs.x, cs.y, cs.z, cs.w}, sw[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float u = x[2 * i] + add[2 * i], w = x[2 * i + 1] + add[2 * i + 1];
+      x[2 * i] = u * cw[i] - w * sw[i];
+      x[2 * i + 1] = w * cw[i] + u * sw[i];
+    }
+  }
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, kv8_mag(x[i]));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const int which = hh >= H + c.Hkv, h = hh - H - which * c.Hkv;    // of a key or value head
+  const int block = p >> c.log2_block, p0 = block << c.log2_block;
+  int8_t* ep = nullptr;
+  int old = KV8_EMIN;
+  if (ok && hh >= H) {
+    ep = (which ? c.ve : c.ke) + b * c.eb + h * c.eh + block;
+    if (p > p0) old = *ep;
+  }
+  __syncwarp();                                                     // the group has read the exponent
+  if (!ok) return;
+  if (hh < H) {
+    *reinterpret_cast<uint4*>(q_out + (static_cast<size_t>(b) * H + hh) * c.D + 8 * j) =
+        make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    return;
+  }
+  const int e = max(kv8_exponent(amax), old);
+  const float inv = pow2i(-e);
+  uint8_t* dst = (which ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(p0) * c.D + 8 * j;
+  *reinterpret_cast<uint2*>(dst + (p - p0) * c.D) = make_uint2(kv8_encode4(x[0], x[1], x[2], x[3], inv), kv8_encode4(x[4], x[5], x[6], x[7], inv));
+  if (j == 0) *ep = static_cast<int8_t>(e);
+  if (p > p0 && e > old) {
+    const float f = pow2i(old - e);
+    for (int t = 0; t < p - p0; ++t) {
+      uint2* w = reinterpret_cast<uint2*>(dst + t * c.D);
+      *w = make_uint2(kv8_recode4(w->x, f), kv8_recode4(w->y, f));
+    }
+  }
+}
+
+// out rows [B * L, ld], head h at column h * D: keys (blockIdx.y 0) and values (1) of positions below L.  With `lens`, positions from the
+// length to the next multiple of 128 become zero (an attention tile that ends there reads them) and later ones are left out.
+__global__ void __launch_bounds__(256)
+kv8_decode_kernel(const Kv8Cache c, const int* __restrict__ lens, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
+                  int L, int most, int ld) {
+  pdl_trigger();
+  pdl_wait();
+  const int vpr = c.D >> 3, per_row = c.Hkv * vpr, b = blockIdx.z;
+  const long long idx = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const int t = static_cast<int>(idx / per_row), col = static_cast<int>(idx - static_cast<long long>(t) * per_row);
+  const int len = lens ? min(max(lens[b], 0), most) : L;
+  if (t >= min(L, (len + 127) & ~127)) return;
+  const int h = col / vpr, d = (col - h * vpr) * 8;
+  uint4 o = make_uint4(0u, 0u, 0u, 0u);
+  if (t < len) {
+    const uint8_t* src = (blockIdx.y ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(t) * c.D + d;
+    const float f = pow2i((blockIdx.y ? c.ve : c.ke)[b * c.eb + h * c.eh + (t >> c.log2_block)]);
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+    const float2 a0 = kv8_float2(w.x, false), a1 = kv8_float2(w.x, true), a2 = kv8_float2(w.y, false), a3 = kv8_float2(w.y, true);
+    o = make_uint4(pack_bf16x2(a0.x * f, a0.y * f), pack_bf16x2(a1.x * f, a1.y * f), pack_bf16x2(a2.x * f, a2.y * f), pack_bf16x2(a3.x * f, a3.y * f));
+  }
+  *reinterpret_cast<uint4*>((blockIdx.y ? v_out : k_out) + (static_cast<long long>(b) * L + t) * ld + h * c.D + d) = o;
+}
+
+// One CTA per (sequence, 256-query tile): {first query token, queries, stream index of the first query, first key of the sequence}, the tiles
+// that see most keys first.  Queries in front of the sequence's first key have nothing to see: they are not in a tile and their outputs
+// become zero here.
+__global__ void __launch_bounds__(256)
+kv8_tiles_kernel(const int* __restrict__ lens, int4* __restrict__ tiles, __nv_bfloat16* __restrict__ out, int n, int most, int L, int per_seq, long long row) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x, i = blockIdx.y, B = gridDim.x;
+  const int len = min(max(lens[b], 0), most), skip = max(0, n - len);  // queries that see nothing
+  const int q = skip + 256 * i, rows = max(0, min(256, n - q));
+  if (threadIdx.x == 0)
+    tiles[(per_seq - 1 - i) * B + b] = make_int4(b * n + (rows ? q : 0), rows, b * L + (rows ? len - n + q : 0), b * L);
+  uint4* o = reinterpret_cast<uint4*>(out + static_cast<long long>(b) * n * row);
+  const long long last = skip * row / 8;
+  for (long long x = static_cast<long long>(i) * 256 + threadIdx.x; x < last; x += 256ll * per_seq) o[x] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+static bool kv8_cache_ok(const Kv8Cache* c) {
+  return c->k && c->v && c->ke && c->ve && c->B > 0 && c->B <= 65535 && c->Hkv > 0 && c->Hkv <= 65535 && c->D >= 32 && c->D <= 128 &&
+         c->D % 32 == 0 && c->log2_block >= 4 && c->log2_block <= 7 && c->cap > 0 && c->cap % (1 << c->log2_block) == 0 &&
+         !((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) && !((c->sb | c->sh) & 15);
+}
+
+// k, v: [B, n, Hkv, D] bf16 with pitches in elements (multiples of eight); start, counts (null: n each): [B].
+B200_API int b200_kv8_append(const Kv8Cache* c, const void* k, const void* v, const long long* pitch, const int* start, const int* counts, int n,
+                             int* err, void* stream) {
+  if (!kv8_cache_ok(c) || n <= 0) return -1;
+  for (int i = 0; i < 6; ++i)
+    if (pitch[i] & 7) return -2;
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
+  const int blk = 1 << c->log2_block;
+  const long long touched = (static_cast<long long>(n) + blk - 2) / blk + 1;
+  const dim3 grid(static_cast<unsigned>(2 * touched), c->Hkv, c->B);
+  const int nv = (blk * (c->D / 8) + 127) / 128;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const __nv_bfloat16 *kb = static_cast<const __nv_bfloat16*>(k), *vb = static_cast<const __nv_bfloat16*>(v);
+#define RUN(NV) launch_k(kv8_append_kernel<NV>, grid, dim3(128), 0, st, *c, kb, vb, pitch[0], pitch[1], pitch[2], pitch[3], pitch[4], pitch[5], start, counts, n, err)
+  if (nv == 1) RUN(1);
+  else if (nv == 2) RUN(2);
+  else if (nv == 3) RUN(3);
+  else if (nv == 4) RUN(4);
+  else if (nv <= 6) RUN(6);
+  else if (nv <= 8) RUN(8);
+  else if (nv <= 12) RUN(12);
+  else RUN(16);
+#undef RUN
+  return cudaGetLastError() == cudaSuccess ? 0 : -10;
+}
+
+// qkv: [B, ld] = [q heads | k heads | v heads], bf16 or fp32; bias: fp32 [(H + Hkv) D] or null; cos / sin: fp32 [>= cap, D / 2]; pos: [B].
+B200_API int b200_kv8_rope_append(const Kv8Cache* c, void* qkv, long long ld, int is_f32, int clear, const float* bias, const float* cosT,
+                                  const float* sinT, const int* pos, void* q_out, int H, int* err, void* stream) {
+  if (!kv8_cache_ok(c) || H <= 0) return -1;
+  if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(cosT) | reinterpret_cast<uintptr_t>(sinT)) & 15) return -2;
+  if (ld & (is_f32 ? 3 : 7)) return -2;
+  const long long units = static_cast<long long>(c->B) * (H + 2 * c->Hkv);
+  if (units > (1ll << 31) - 16) return -3;
+  const dim3 grid(static_cast<unsigned>((units + 15) / 16));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  __nv_bfloat16* qo = static_cast<__nv_bfloat16*>(q_out);
+  if (is_f32) launch_k(kv8_rope_append_kernel<true>, grid, dim3(256), 0, st, *c, qkv, ld, bias, cosT, sinT, pos, qo, H, clear, err);
+  else launch_k(kv8_rope_append_kernel<false>, grid, dim3(256), 0, st, *c, qkv, ld, bias, cosT, sinT, pos, qo, H, clear, err);
+  return cudaGetLastError() == cudaSuccess ? 0 : -10;
+}
+
+// k_out, v_out: bf16 [B, L, Hkv, D] contiguous, lens: see kv8_decode_kernel (no length counts for more than `most`).
+B200_API int b200_kv8_decode(const Kv8Cache* c, const int* lens, void* k_out, void* v_out, int L, int most, void* stream) {
+  if (!kv8_cache_ok(c) || L <= 0 || most > L || most > c->cap || (!lens && L > c->cap)) return -1;
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return -2;
+  const long long vecs = static_cast<long long>(L) * c->Hkv * (c->D / 8);
+  if (vecs > (1ll << 38)) return -3;
+  launch_k(kv8_decode_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256), 2, c->B), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), *c, lens,
+           static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), L, most, c->Hkv * c->D);
+  return cudaGetLastError() == cudaSuccess ? 0 : -10;
+}
+
+// tiles: int4 [B * ceil(n / 256)]; out: bf16 [B, n, row]; most: no length is larger (larger ones are cut), L: key rows per sequence.
+B200_API int b200_kv8_tiles(const int* lens, int* tiles, void* out, int B, int n, int most, int L, long long row, void* stream) {
+  const int per_seq = (n + 255) / 256;
+  if (B <= 0 || n <= 0 || per_seq > 65535 || most > L || (row & 7)) return -1;
+  launch_k(kv8_tiles_kernel, dim3(B, per_seq), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), lens, reinterpret_cast<int4*>(tiles),
+           static_cast<__nv_bfloat16*>(out), n, most, L, per_seq, row);
+  return cudaGetLastError() == cudaSuccess ? 0 : -10;
+}

@@ -1,0 +1,278 @@
+"""Operators of an 8-bit key / value cache: CUDA tensors run the kernels of ``csrc/kv8.cu`` and ``csrc/kv8_attention.cu`` (long
+prompts: ``csrc/latent_attention.cu`` behind a pass that turns codes into bf16), CPU tensors the plain statements of ``reference``.
+A CUDA tensor never takes the plain path.
+
+The cache holds e4m3 codes ``[B, kv_heads, capacity, dim]`` and one int8 exponent per head and block of tokens ``[B, kv_heads,
+capacity / block]``; a value is ``code * 2**exponent``.  The exponent of a block is the least that brings its largest magnitude to
+448 or less; it never falls below -40, so values below 2**-49 are stored as zero.  A position's block is begun when its
+first position is written, so rows of an earlier sequence need no clearing; a sequence is written in order, and writing at a position
+again forgets what lies behind it in the block.  Infinities are stored as the block's largest code, NaN as NaN.
+
+Sequences are described by int32 tensors on the cache's device and never read by the host: a position or length outside the cache is
+left out by the kernels (nothing is written; lengths are cut to the capacity) and recorded in the device status word
+(``cuda.check_device_status``).  Calls run on the current stream and allocate through PyTorch's allocator."""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import reference as ref
+
+BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+BLOCKS = (16, 32, 64, 128)
+STREAM_ROWS = 64        # query tokens x heads per key head up to which the cache is streamed as it is
+
+
+class _Cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ke", "ve")] + [(n, C.c_longlong) for n in ("sb", "sh", "eb", "eh")] + \
+               [(n, C.c_int) for n in ("B", "Hkv", "cap", "D", "log2_block")]
+
+
+class _Attn(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ke", "ve")] + [(n, C.c_longlong) for n in ("sb", "sh", "eb", "eh")] + \
+               [(n, C.c_int) for n in ("B", "Hkv", "cap", "D", "log2_block")] + [("q", C.c_void_p)] + \
+               [(n, C.c_longlong) for n in ("q_sb", "q_sn", "q_sh")] + [(n, C.c_void_p) for n in ("lens", "out", "part")] + \
+               [(n, C.c_int) for n in ("n", "group", "rows", "tiles_r", "tile", "most")] + [("scale_log2", C.c_float)]
+
+
+_fns = None
+
+
+def _k():
+    global _fns
+    if _fns is None:
+        from types import SimpleNamespace
+
+        from . import cuda as K
+
+        vp, i, ll = C.c_void_p, C.c_int, C.c_longlong
+        _fns = SimpleNamespace(
+            K=K,
+            append=K._sig("b200_kv8_append", [C.POINTER(_Cache), vp, vp, C.POINTER(ll), vp, vp, i, vp, vp]),
+            rope=K._sig("b200_kv8_rope_append", [C.POINTER(_Cache), vp, ll, i, i, vp, vp, vp, vp, vp, i, vp, vp]),
+            decode=K._sig("b200_kv8_decode", [C.POINTER(_Cache), vp, vp, vp, i, i, vp]),
+            tiles=K._sig("b200_kv8_tiles", [vp, vp, vp, i, i, i, i, ll, vp]),
+            plan=K._sig("b200_kv8_attention_plan", [i] * 5 + [C.POINTER(i)]),
+            attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn), i, vp]),
+            long_ok=K._sig("b200_capped_attention_supported", [i, i]),
+            long=K._sig("b200_capped_attention", [vp] * 6 + [i] * 12 + [C.c_float] * 3 + [vp, vp]),
+        )
+    return _fns
+
+
+class _On:
+    """Makes a tensor's device the current one around a launch."""
+
+    def __init__(self, device):
+        self.guard = None if device.index is None or device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+@dataclass(eq=False)
+class KV8Cache:
+    """Codes and exponents of one layer's keys and values.  The tensors may be views (of a cache with more slots, say): a head's
+    positions and channels have to be contiguous, codes and exponents of keys and values laid out alike."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: torch.Tensor
+    v_exp: torch.Tensor
+
+    def __post_init__(self):
+        k, v, ke, ve = self.k, self.v, self.k_exp, self.v_exp
+        if k.dim() != 4 or k.dtype != E4M3 or v.dtype != E4M3 or v.shape != k.shape:
+            raise ValueError("codes are two float8_e4m3fn tensors [B, kv_heads, capacity, dim]")
+        if ke.dim() != 3 or ke.dtype != torch.int8 or ve.dtype != torch.int8 or ve.shape != ke.shape or ke.shape[:2] != k.shape[:2]:
+            raise ValueError("exponents are two int8 tensors [B, kv_heads, capacity / block]")
+        if len({t.device for t in (k, v, ke, ve)}) != 1:
+            raise ValueError("codes and exponents lie on one device")
+        self.batch, self.kv_heads, self.capacity, self.dim = k.shape
+        blocks = ke.shape[2]
+        self.block = self.capacity // blocks if blocks else 0
+        if self.block not in BLOCKS or self.block * blocks != self.capacity:
+            raise ValueError(f"blocks of {BLOCKS} tokens: got {blocks} exponents for {self.capacity} positions")
+        if self.dim % 32 or not 32 <= self.dim <= 128:
+            raise ValueError(f"head dims of 32, 64, 96 and 128: got {self.dim}")
+        if min(k.shape) == 0:
+            raise ValueError("a cache has at least one sequence, head and position")
+        if k.stride()[2:] != (self.dim, 1) or v.stride() != k.stride() or ke.stride(2) != 1 or ve.stride() != ke.stride():
+            raise ValueError("a head's positions are contiguous, and keys and values laid out alike")
+        if k.is_cuda and ((k.data_ptr() | v.data_ptr() | k.stride(0) | k.stride(1)) & 15):
+            raise ValueError("heads start on 16-byte boundaries")
+        self.device = k.device
+        self._c = _Cache(k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), k.stride(0), k.stride(1), ke.stride(0), ke.stride(1),
+                         *k.shape, self.block.bit_length() - 1)
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, capacity: int, dim: int, device=None, block: int = 32) -> "KV8Cache":
+        """A cache for ``capacity`` positions (rounded up to whole blocks) per sequence."""
+        if block not in BLOCKS:
+            raise ValueError(f"blocks of {BLOCKS} tokens: got {block}")
+        n = (capacity + block - 1) // block
+        codes = [torch.zeros(batch, kv_heads, n * block, dim, dtype=torch.uint8, device=device).view(E4M3) for _ in range(2)]
+        return cls(*codes, *(torch.full((batch, kv_heads, n), ref.KV8_EMIN, dtype=torch.int8, device=device) for _ in range(2)))
+
+    def decoded(self) -> tuple:
+        """Keys and values of all positions as bf16 [B, capacity, kv_heads, dim] (exact)."""
+        if not self.k.is_cuda:
+            return tuple(ref.kv8_decode(c, e).transpose(1, 2).to(BF16) for c, e in ((self.k, self.k_exp), (self.v, self.v_exp)))
+        k, v = (torch.empty(self.batch, self.capacity, self.kv_heads, self.dim, dtype=BF16, device=self.device) for _ in range(2))
+        f = _k()
+        with _On(self.device):
+            f.K._check(f.decode(C.byref(self._c), 0, k.data_ptr(), v.data_ptr(), self.capacity, self.capacity, f.K._stream()), "kv8_decode")
+        return k, v
+
+
+def _index(t: torch.Tensor, cache: KV8Cache, what: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.shape != (cache.batch,) or t.device != cache.device or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 tensor [{cache.batch}] on the cache's device")
+    return t
+
+
+def _pitch(x: torch.Tensor) -> list:
+    """Strides of all but the last dimension; those of single entries do not matter."""
+    return [0 if n == 1 else st for n, st in zip(x.shape[:-1], x.stride())]
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x, copied unless its head vectors are contiguous and start on 16-byte boundaries."""
+    if x.stride(-1) == 1 and not (x.data_ptr() & 15) and not any(s & 7 for s in _pitch(x)):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
+    """Write keys and values [B, n, kv_heads, dim] (bf16, any pitches) of positions ``start[b] .. start[b] + n - 1`` into the cache;
+    ``counts``: only the first ``counts[b]`` of a sequence's n."""
+    if k.dim() != 4 or k.dtype != BF16 or v.dtype != BF16 or k.shape != v.shape or k.device != cache.device or v.device != cache.device:
+        raise ValueError("keys and values are bf16 [B, n, kv_heads, dim] on the cache's device")
+    B, n, H, D = k.shape
+    if (B, H, D) != (cache.batch, cache.kv_heads, cache.dim):
+        raise ValueError(f"keys {tuple(k.shape)} do not fit a cache of {cache.batch} sequences, {cache.kv_heads} heads of {cache.dim}")
+    _index(start, cache, "start")
+    if counts is not None:
+        _index(counts, cache, "counts")
+    if n == 0:
+        return
+    if not k.is_cuda:
+        return ref.kv8_append(cache, k, v, start, counts)
+    f = _k()
+    k, v = _rows(k), _rows(v)
+    pitch = (C.c_longlong * 6)(*_pitch(k), *_pitch(v))
+    with _On(cache.device):
+        f.K._check(f.append(C.byref(cache._c), k.data_ptr(), v.data_ptr(), pitch, start.data_ptr(), f.K._ptr(counts), n,
+                            f.K.err_word(cache.device).data_ptr(), f.K._stream()), "kv8_append")
+
+
+def rope_append(cache: KV8Cache, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, heads: int,
+                bias: Optional[torch.Tensor] = None, clear: bool = False) -> torch.Tensor:
+    """The new token of every sequence: ``qkv`` [B, (heads + 2 kv_heads) dim] (bf16 or fp32) holds its packed projection.  Adds the fp32
+    ``bias`` [(heads + kv_heads) dim] to q and k, turns their neighbouring pairs by the angles of position ``pos[b]`` (``cos`` / ``sin``: fp32
+    [>= capacity, dim / 2]), writes k and v into the cache and returns q as bf16 [B, heads, dim].  Rows whose position lies outside the
+    cache keep an undefined q.  ``clear`` hands an fp32 ``qkv`` back zeroed (the accumulator of a decode step's product)."""
+    B, D, Hkv = cache.batch, cache.dim, cache.kv_heads
+    W = (heads + 2 * Hkv) * D
+    if heads <= 0 or heads % Hkv:
+        raise ValueError(f"{heads} query heads do not share {Hkv} key heads evenly")
+    if qkv.dim() != 2 or tuple(qkv.shape) != (B, W) or qkv.dtype not in (BF16, F32) or qkv.device != cache.device or qkv.stride(1) != 1:
+        raise ValueError(f"qkv is bf16 or fp32 [{B}, {W}] with contiguous rows on the cache's device")
+    for t, what in ((cos, "cos"), (sin, "sin")):
+        if t.dtype != F32 or t.dim() != 2 or t.shape[1] != D // 2 or t.shape[0] < cache.capacity or not t.is_contiguous() or t.device != cache.device:
+            raise ValueError(f"{what} is a contiguous fp32 table [>= {cache.capacity}, {D // 2}] on the cache's device")
+    if bias is not None and (bias.dtype != F32 or bias.numel() != (heads + Hkv) * D or not bias.is_contiguous() or bias.device != cache.device):
+        raise ValueError(f"bias is a contiguous fp32 tensor of {(heads + Hkv) * D} values on the cache's device")
+    if clear and qkv.dtype != F32:
+        raise ValueError("only an fp32 accumulator is handed back zeroed")
+    _index(pos, cache, "pos")
+    if not qkv.is_cuda:
+        return ref.kv8_rope_append(cache, qkv, cos, sin, pos, heads, bias, clear)
+    f = _k()
+    if (qkv.data_ptr() & 15) or (qkv.stride(0) * qkv.element_size() & 15):
+        if clear:
+            raise ValueError("an accumulator that is cleared has rows on 16-byte boundaries")
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    if (cos.data_ptr() | sin.data_ptr()) & 15:
+        cos, sin = cos.clone(), sin.clone()
+    q = torch.empty(B, heads, D, dtype=BF16, device=cache.device)
+    with _On(cache.device):
+        f.K._check(f.rope(C.byref(cache._c), qkv.data_ptr(), qkv.stride(0), qkv.dtype == F32, clear, f.K._ptr(bias), cos.data_ptr(), sin.data_ptr(),
+                          pos.data_ptr(), q.data_ptr(), heads, f.K.err_word(cache.device).data_ptr(), f.K._stream()), "kv8_rope_append")
+    return q
+
+
+_plans: dict = {}
+
+
+def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optional[float] = None, max_len: Optional[int] = None) -> torch.Tensor:
+    """Causal attention of each sequence's n newest tokens: ``q`` [B, n, heads, dim] (bf16), the last one sees the first ``lens[b]`` positions
+    of the cache, the one before it one fewer, and so on; one that sees nothing gets zeros.  Returns bf16 [B, n, heads, dim].
+    ``scale``: factor of the scores, dim ** -0.5 by default.  ``max_len``: no length is larger (longer ones are cut); the capacity by
+    default.  A smaller bound makes short calls cheaper."""
+    if q.dim() != 4 or q.dtype != BF16 or q.device != cache.device:
+        raise ValueError("q is bf16 [B, n, heads, dim] on the cache's device")
+    B, n, H, D = q.shape
+    if (B, D) != (cache.batch, cache.dim) or H == 0 or H % cache.kv_heads:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {cache.batch} sequences, {cache.kv_heads} heads of {cache.dim}")
+    _index(lens, cache, "lens")
+    most = cache.capacity if max_len is None else int(max_len)
+    if not 0 < most <= cache.capacity:
+        raise ValueError(f"max_len lies in 1 .. {cache.capacity}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if n == 0:
+        return torch.empty_like(q)
+    if not q.is_cuda:
+        return ref.kv8_attention(q, cache, lens, scale, most)
+    group = H // cache.kv_heads
+    q = _rows(q)
+    if n * group > STREAM_ROWS and scale > 0:
+        return _long(q, cache, lens, scale, most)
+    f = _k()
+    out = torch.empty(B, n, H, D, dtype=BF16, device=cache.device)
+    with _On(cache.device):
+        key = (cache.device.index, B, cache.kv_heads, D, n * group, most)
+        plan = _plans.get(key)
+        if plan is None:
+            buf = (C.c_int * 5)()
+            rc = f.plan(B, cache.kv_heads, D, n * group, most, buf)
+            if rc:
+                raise RuntimeError(f"kv8_attention_plan failed with code {rc}")
+            plan = _plans[key] = tuple(buf)
+        rows, tiles_r, tile, ctas, scratch = plan
+        part = torch.empty(scratch, dtype=F32, device=cache.device) if scratch else None
+        c = cache._c
+        p = _Attn(c.k, c.v, c.ke, c.ve, c.sb, c.sh, c.eb, c.eh, B, c.Hkv, c.cap, D, c.log2_block, q.data_ptr(), *_pitch(q), lens.data_ptr(),
+                  out.data_ptr(), f.K._ptr(part), n, group, rows, tiles_r, tile, most, scale * 1.4426950408889634)
+        f.K._check(f.attn(C.byref(p), ctas, f.K._stream()), "kv8_attention")
+    return out
+
+
+def _long(q, cache, lens, scale, most) -> torch.Tensor:
+    """Many query rows per key: the codes become bf16 rows once (exactly), and the prompt attention on the tensor cores reads those."""
+    f = _k()
+    B, n, H, D = q.shape
+    Hkv, W = cache.kv_heads, cache.kv_heads * D
+    L = (most + 127) // 128 * 128
+    q = q if q.is_contiguous() else q.contiguous()
+    per = (n + 255) // 256
+    if B * per > 65535 or B * max(L, n) >= 2 ** 31:
+        raise ValueError(f"{B} sequences of {n} tokens and {most} keys are too many for one call")
+    with _On(cache.device):
+        K, st = f.K, f.K._stream()
+        out = torch.empty(B, n, H, D, dtype=BF16, device=cache.device)
+        kv = torch.empty(2, B * L, W, dtype=BF16, device=cache.device)
+        tiles = torch.empty(B * per, 4, dtype=torch.int32, device=cache.device)
+        K._check(f.decode(C.byref(cache._c), lens.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), L, most, st), "kv8_decode")
+        K._check(f.tiles(lens.data_ptr(), tiles.data_ptr(), out.data_ptr(), B, n, most, L, H * D, st), "kv8_tiles")
+        K._check(f.long(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), 0, B * per, B * n, B * L, H, Hkv, D, D,
+                        H * D, W, H * D, 2 ** 30, 0, scale, 0.0, 0.0, st, K.err_word(cache.device).data_ptr()), "capped_attention")
+    return out

@@ -325,3 +325,117 @@ def route_grouped(z: torch.Tensor, top: int, groups: int, keep: int):
     allowed = torch.zeros_like(strength, dtype=torch.bool).scatter_(1, best, True)[:, :, None].expand_as(g).flatten(1)
     idx = torch.sort(s.masked_fill(~allowed, float("-inf")), dim=-1, descending=True, stable=True).indices[:, :top]
     return idx, s.gather(1, idx)
+
+
+# ------------------------------------------------------------------------------------------
+# 8-bit key / value cache, sampling from given numbers
+# ------------------------------------------------------------------------------------------
+KV8_EMIN, KV8_EMAX, KV8_MAX = -40, 119, 448.0
+
+
+def kv8_exponent(amax: torch.Tensor) -> torch.Tensor:
+    """The least exponent (within the stored range) that brings ``amax`` to the largest e4m3 value, 448, or less."""
+    mant, e = torch.frexp(amax.double())               # amax = mant 2^e, mant in [1/2, 1);  448 = 7/8 2^9
+    e = torch.where(mant > 0.875, e - 8, e - 9)
+    return torch.where(amax > 0, e, KV8_EMIN).clamp(KV8_EMIN, KV8_EMAX)
+
+
+def kv8_encode(x: torch.Tensor, e: torch.Tensor) -> torch.Tensor:
+    """Codes of fp32 values under exponents ``e`` (broadcast): to nearest, infinities as the largest code, NaN as NaN."""
+    return torch.ldexp(x.double(), -e).clamp(-KV8_MAX, KV8_MAX).float().to(torch.float8_e4m3fn)
+
+
+def kv8_decode(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    """fp32 values of codes [..., T, D] with exponents [..., T / block]."""
+    return torch.ldexp(codes.float(), exps.int().repeat_interleave(codes.shape[-2] // exps.shape[-1], -1)[..., None])
+
+
+def _kv8_put(codes, exps, x, start: int, block: int) -> None:
+    """One sequence: positions start .. of codes [H, cap, D] become x [n, H, D] (fp32), block by block."""
+    raw = codes.view(torch.uint8)
+    for lo in range(start - start % block, start + x.shape[0], block):
+        a, z = max(lo, start), min(lo + block, start + x.shape[0])
+        new = x[a - start:z - start].transpose(0, 1)
+        e = kv8_exponent(torch.where(torch.isfinite(new), new.abs(), 0.0).amax((1, 2)))
+        if a > lo:                                      # the block goes on: the larger exponent, older codes under it
+            old = exps[:, lo // block].int()
+            e = torch.maximum(e, old)
+            raw[:, lo:a] = kv8_encode(torch.ldexp(codes[:, lo:a].float(), old[:, None, None]), e[:, None, None]).view(torch.uint8)
+        raw[:, a:z] = kv8_encode(new, e[:, None, None]).view(torch.uint8)
+        exps[:, lo // block] = e.to(torch.int8)
+
+
+def kv8_append(cache, k, v, start, counts=None) -> None:
+    """Positions start[b] .. of the cache become the first counts[b] tokens of k, v [B, n, Hkv, D]; a sequence that does not fit is left out."""
+    n = k.shape[1]
+    for b, at in enumerate(start.tolist()):
+        c = n if counts is None else int(counts[b])
+        if at < 0 or not 0 <= c <= n or at + c > cache.capacity or c == 0:
+            continue
+        _kv8_put(cache.k[b], cache.k_exp[b], k[b, :c].float(), at, cache.block)
+        _kv8_put(cache.v[b], cache.v_exp[b], v[b, :c].float(), at, cache.block)
+
+
+def kv8_rope_append(cache, qkv, cos, sin, pos, heads, bias=None, clear=False) -> torch.Tensor:
+    """Bias, rotation of neighbouring pairs and cache append of one new token per sequence, in fp32; q rounded once."""
+    B, D, Hkv = cache.batch, cache.dim, cache.kv_heads
+    x = qkv.float().view(B, heads + 2 * Hkv, D)
+    qk, v = x[:, :heads + Hkv], x[:, heads + Hkv:]
+    if bias is not None:
+        qk = qk + bias.view(heads + Hkv, D)
+    ok = (pos >= 0) & (pos < cache.capacity)
+    at = torch.where(ok, pos, 0).long()
+    qk = rope_interleaved(qk[:, None], cos[at][:, None, None], sin[at][:, None, None])[:, 0]
+    for b in range(B):
+        if ok[b]:
+            _kv8_put(cache.k[b], cache.k_exp[b], qk[b:b + 1, heads:], int(pos[b]), cache.block)
+            _kv8_put(cache.v[b], cache.v_exp[b], v[b:b + 1], int(pos[b]), cache.block)
+    q = qk[:, :heads].to(torch.bfloat16)
+    if clear:
+        qkv.zero_()
+    return q
+
+
+def kv8_attention(q, cache, lens, scale: float, max_len: int) -> torch.Tensor:
+    """Query i of n sees the first lens[b] - (n - 1 - i) positions of the cache; without any its output is zero."""
+    B, n, H, D = q.shape
+    out = torch.zeros(B, n, H, D, dtype=torch.float32, device=q.device)
+    group = H // cache.kv_heads
+    for b, L in enumerate(lens.tolist()):
+        L = min(max(L, 0), max_len)
+        k, v = (kv8_decode(c[b], e[b])[:, :L].repeat_interleave(group, 0) for c, e in ((cache.k, cache.k_exp), (cache.v, cache.v_exp)))
+        for i in range(n):
+            m = L - (n - 1 - i)
+            if m > 0:
+                w = torch.softmax(torch.einsum("hd,hkd->hk", q[b, i].float(), k[:, :m]) * scale, -1)
+                out[b, i] = torch.einsum("hk,hkd->hd", w, v[:, :m])
+    return out.to(q.dtype)
+
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
+    """One token per row; see ``ops.sampling.sample_tokens``.  Numbers are taken as fp32, as a row's own setting would be."""
+    x = torch.where(torch.isnan(logits), -math.inf, logits.double())
+    B, V = x.shape
+
+    def row(a):
+        a = a if torch.is_tensor(a) else torch.full((B,), float(a), dtype=torch.float32, device=x.device)
+        return a.double()[:, None]
+
+    t, p, m = row(temperature), row(top_p), row(min_p).clamp_max(1.0)
+    k = (top_k if torch.is_tensor(top_k) else torch.full((B,), top_k, device=x.device)).long()[:, None]
+    xs, order = torch.sort(x, dim=-1, descending=True, stable=True)
+    top = xs[:, :1]
+    d = torch.where(xs == top, 0.0, top - xs)
+    w = torch.exp(-torch.where(d > 0, d / torch.where(t > 0, t, 1.0), 0.0))
+    keep = (k <= 0) | (xs >= xs.gather(1, k.clamp(1, V) - 1))
+    prefix = w.cumsum(-1) <= p * w.sum(-1, keepdim=True)
+    prefix[:, 0] = True
+    keep &= prefix | (p <= 0) | (p >= 1)
+    keep &= (m <= 0) | (w >= m)
+    kept = torch.zeros_like(w).scatter(1, order, torch.where(keep, w, 0.0)).cumsum(-1)
+    u = torch.nan_to_num(uniform.double(), nan=0.0).clamp_min(0.0)
+    hit = kept > u[:, None] * kept[:, -1:]
+    last = torch.where(keep, order, -1).amax(-1)         # a number of 1 or more: the last kept token
+    token = torch.where(hit.any(-1), hit.int().argmax(-1), last)
+    token = torch.where(t[:, 0] > 0, token, order[:, 0])
+    return torch.where(top[:, 0] == -math.inf, -1, token)
