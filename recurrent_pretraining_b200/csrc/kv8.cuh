@@ -15,11 +15,13 @@ constexpr int KV8_EMIN = -40, KV8_EMAX = 119;
 
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((max(e, -126) + 127) << 23); }   // e <= 127
 
-// The least exponent that brings `amax` (finite, >= 0) to at most 448 = 0.875 * 2^9.
-__device__ __forceinline__ int kv8_exponent(float amax) {
+// The least exponent that brings `amax` (finite, > 0) to at most 448 = 0.875 * 2^9; as far as it is stored.
+__device__ __forceinline__ int kv8_exponent_any(float amax) {
   const int bits = __float_as_int(amax);
-  const int e = (bits >> 23) - 126 - 9 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0);
-  return amax > 0.f ? min(max(e, KV8_EMIN), KV8_EMAX) : KV8_EMIN;
+  return (bits >> 23) - 126 - 9 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0);
+}
+__device__ __forceinline__ int kv8_exponent(float amax) {
+  return amax > 0.f ? min(max(kv8_exponent_any(amax), KV8_EMIN), KV8_EMAX) : KV8_EMIN;
 }
 // Magnitude that counts for a block's exponent: infinities (stored as the largest code) and NaN (stored as NaN) do not.
 __device__ __forceinline__ float kv8_mag(float x) {
@@ -34,8 +36,9 @@ __device__ __forceinline__ uint32_t kv8_encode4(float a, float b, float c, float
 }
 // Two codes -> f16x2 (exact); `hi`: the upper two of the word.
 __device__ __forceinline__ uint32_t kv8_half2(uint32_t w, bool hi) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(hi ? w >> 16 : w & 0xFFFF), __NV_E4M3);
-  return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<unsigned short>(hi ? w >> 16 : w)));
+  return h;
 }
 __device__ __forceinline__ float2 kv8_float2(uint32_t w, bool hi) {
   const uint32_t h = kv8_half2(w, hi);

@@ -35,7 +35,7 @@ class _Attn(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ke", "ve")] + [(n, C.c_longlong) for n in ("sb", "sh", "eb", "eh")] + \
                [(n, C.c_int) for n in ("B", "Hkv", "cap", "D", "log2_block")] + [("q", C.c_void_p)] + \
                [(n, C.c_longlong) for n in ("q_sb", "q_sn", "q_sh")] + [(n, C.c_void_p) for n in ("lens", "out", "part")] + \
-               [(n, C.c_int) for n in ("n", "group", "rows", "tiles_r", "tile", "most")] + [("scale_log2", C.c_float)]
+               [(n, C.c_int) for n in ("n", "group", "rows", "tiles_r", "most")] + [("scale_log2", C.c_float), ("ctas", C.c_int)]
 
 
 _fns = None
@@ -56,7 +56,7 @@ def _k():
             decode=K._sig("b200_kv8_decode", [C.POINTER(_Cache), vp, vp, vp, i, i, vp]),
             tiles=K._sig("b200_kv8_tiles", [vp, vp, vp, i, i, i, i, ll, vp]),
             plan=K._sig("b200_kv8_attention_plan", [i] * 5 + [C.POINTER(i)]),
-            attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn), i, vp]),
+            attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn), vp]),
             long_ok=K._sig("b200_capped_attention_supported", [i, i]),
             long=K._sig("b200_capped_attention", [vp] * 6 + [i] * 12 + [C.c_float] * 3 + [vp, vp]),
         )
@@ -242,17 +242,17 @@ def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optio
         key = (cache.device.index, B, cache.kv_heads, D, n * group, most)
         plan = _plans.get(key)
         if plan is None:
-            buf = (C.c_int * 5)()
+            buf = (C.c_int * 4)()
             rc = f.plan(B, cache.kv_heads, D, n * group, most, buf)
             if rc:
                 raise RuntimeError(f"kv8_attention_plan failed with code {rc}")
             plan = _plans[key] = tuple(buf)
-        rows, tiles_r, tile, ctas, scratch = plan
-        part = torch.empty(scratch, dtype=F32, device=cache.device) if scratch else None
+        rows, tiles_r, ctas, scratch = plan
+        part = torch.empty(scratch, dtype=F32, device=cache.device)
         c = cache._c
         p = _Attn(c.k, c.v, c.ke, c.ve, c.sb, c.sh, c.eb, c.eh, B, c.Hkv, c.cap, D, c.log2_block, q.data_ptr(), *_pitch(q), lens.data_ptr(),
-                  out.data_ptr(), f.K._ptr(part), n, group, rows, tiles_r, tile, most, scale * 1.4426950408889634)
-        f.K._check(f.attn(C.byref(p), ctas, f.K._stream()), "kv8_attention")
+                  out.data_ptr(), part.data_ptr(), n, group, rows, tiles_r, most, scale * 1.4426950408889634, ctas)
+        f.K._check(f.attn(C.byref(p), f.K._stream()), "kv8_attention")
     return out
 
 
