@@ -227,7 +227,7 @@ static bool kv8_cache_ok(const Kv8Cache* c) {
          !((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) && !((c->sb | c->sh) & 15);
 }
 
-// k, v: [B, n, Hkv, D] bf16 with pitches in elements (multiples of eight); start, counts (null: n each): [B].
+// k, v: [B, n, Hkv, D] bf16 with pitches in elements (three each, multiples of eight); start, counts (null: n each): [B].
 B200_API int b200_kv8_append(const Kv8Cache* c, const void* k, const void* v, const long long* pitch, const int* start, const int* counts, int n,
                              int* err, void* stream) {
   if (!kv8_cache_ok(c) || n <= 0) return -1;

@@ -42,6 +42,7 @@ struct Kv8Attn {
   int most;                          // no length counts for more
   float scale_log2;
   int ctas;
+  uint32_t group_magic;              // ceil(2^32 / group)
 };
 
 constexpr int KA_WARPS = 4, KA_STEP = 32;           // keys per warp and step
@@ -79,6 +80,9 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+
+// Token of a row (row / group for rows up to 2^32 / group).
+__device__ __forceinline__ int kv8_token(const Kv8Attn& p, int row) { return p.group == 1 ? row : static_cast<int>(__umulhi(row, p.group_magic)); }
 
 // Where the steps of every sequence lie and which warp takes which of them (the first total % G take one more than the others); the
 // same arithmetic in both kernels.  Every warp holds the lengths of 32 sequences, one per lane.
@@ -255,9 +259,6 @@ kv8_attention_kernel(const Kv8Attn p) {
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll 1
-  for (int i = 0; i < ST - 1; ++i) request(i);
-
   // What a range begins with is loaded while the one before it is worked on: q rows (lane g: row g of a column tile), exponents of the first
   // step and of the sequence's first block of values.
   uint2 q_raw[NT == 1 ? 2 * KS : 1];
@@ -273,7 +274,7 @@ kv8_attention_kernel(const Kv8Attn p) {
   auto q_load = [&](const Range& r, int c8, uint2* raw) {
     const int x = r.r0 + 8 * c8 + g;
     const bool real = 8 * c8 + g < min(p.rows, p.n * p.group - r.r0);
-    const int i = real && p.n > 1 ? x / p.group : 0, hq = r.h * p.group + (real ? x - i * p.group : 0);
+    const int i = real && p.n > 1 ? kv8_token(p, x) : 0, hq = r.h * p.group + (real ? x - i * p.group : 0);
     const __nv_bfloat16* qp = p.q + r.b * p.q_sb + i * p.q_sn + hq * p.q_sh + 4 * t;
 #pragma unroll
     for (int j = 0; j < 2 * KS; ++j) raw[j] = real ? __ldg(reinterpret_cast<const uint2*>(qp + 16 * j)) : make_uint2(0u, 0u);
@@ -317,7 +318,9 @@ kv8_attention_kernel(const Kv8Attn p) {
     }
   };
   nxt.next(p, sh, hi);
-  prepare(nxt);
+  prepare(nxt);                                     // in front of the bulk of the requests
+#pragma unroll 1
+  for (int i = 0; i < ST - 1; ++i) request(i);
   if (p.n > 1)
     for (int d = lane; d < D; d += 32) nan_key[d] = INT_MAX;
   int stage = 0;
@@ -337,11 +340,12 @@ kv8_attention_kernel(const Kv8Attn p) {
       colf[0][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
     } else {
       __syncwarp();
+      uint2 raw[NT][2 * KS];                        // all of them on their way together
+#pragma unroll
+      for (int c8 = 0; c8 < NT; ++c8) q_load(now, c8, raw[c8]);
 #pragma unroll
       for (int c8 = 0; c8 < NT; ++c8) {
-        uint2 raw[2 * KS];
-        q_load(now, c8, raw);
-        const float f = q_convert(raw, sm_q + c8 * KS * 32 + lane, 32);
+        const float f = q_convert(raw[c8], sm_q + c8 * KS * 32 + lane, 32);
         if (t == 0) sm_f[8 * c8 + g] = f;
       }
       __syncwarp();
@@ -364,8 +368,9 @@ kv8_attention_kernel(const Kv8Attn p) {
     for (int c8 = 0; c8 < NT; ++c8)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        limit[c8][i] = p.n == 1 ? key1 : min(key1, len - (p.n - 1) + min((r0 + 8 * c8 + 2 * t + i) / p.group, p.n - 1));
+        limit[c8][i] = p.n == 1 ? key1 : min(key1, len - (p.n - 1) + min(kv8_token(p, r0 + 8 * c8 + 2 * t + i), p.n - 1));
 
+    bool noted = false;                             // a NaN of V that only some rows see
     float o[VB][NT][4], R[NT][2], l[NT][2];
 #pragma unroll
     for (int c8 = 0; c8 < NT; ++c8) {
@@ -441,11 +446,11 @@ kv8_attention_kernel(const Kv8Attn p) {
         float mx[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) mx[i] = fmaxf(fmaxf(s[0][c8][i], s[0][c8][i + 2]), fmaxf(s[1][c8][i], s[1][c8][i + 2]));
+        if (__any_sync(0xffffffffu, mx[0] > R[c8][0] || mx[1] > R[c8][1])) {    // seldom after the first steps
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1)
+          for (int x = 4; x < 32; x <<= 1)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], x));
-        if (__any_sync(0xffffffffu, mx[0] > R[c8][0] || mx[1] > R[c8][1])) {
+            for (int i = 0; i < 2; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], x));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float rn = fmaxf(R[c8][i], mx[i]), alpha = ex2_approx(R[c8][i] - rn);
@@ -483,6 +488,7 @@ kv8_attention_kernel(const Kv8Attn p) {
           for (int i = 0; i < 4; ++i) {
             const uint32_t nan = ((v[w][i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
             if (nan) {
+              noted = true;
               for (int y = 0; y < 4; ++y)
                 if (nan >> (8 * y + 7) & 1u) {
                   atomicMin(&nan_key[16 * w + g + 8 * (i & 1)], key + 16 * (i >> 1) + 4 * t + y);
@@ -504,7 +510,7 @@ kv8_attention_kernel(const Kv8Attn p) {
 
     // ---- the range's outputs, or this share's part of them
     const bool whole = now.begins && now.ends;
-    if (p.n > 1) __syncwarp();                      // NaNs noted by other lanes
+    noted = __any_sync(0xffffffffu, noted);
 #pragma unroll
     for (int c8 = 0; c8 < NT; ++c8)
 #pragma unroll
@@ -514,8 +520,8 @@ kv8_attention_kernel(const Kv8Attn p) {
         for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         const int c = 8 * c8 + 2 * t + i;
         if (c < nrows) {
-          const int row = r0 + c, tok = p.n == 1 ? 0 : row / p.group, hq = now.h * p.group + row - tok * p.group;
-          if (p.n > 1) {
+          const int row = r0 + c, tok = p.n == 1 ? 0 : kv8_token(p, row), hq = now.h * p.group + row - tok * p.group;
+          if (noted) {
             const int sees = len - (p.n - 1) + tok;
 #pragma unroll
             for (int w = 0; w < VB; ++w) {
@@ -542,7 +548,7 @@ kv8_attention_kernel(const Kv8Attn p) {
           }
         }
       }
-    if (p.n > 1) {
+    if (noted) {
       __syncwarp();
       for (int d = lane; d < D; d += 32) nan_key[d] = INT_MAX;
       __syncwarp();
@@ -710,13 +716,19 @@ B200_API int b200_kv8_attention_plan(int B, int Hkv, int D, int rows, int most, 
   return 0;
 }
 
-// p as in Kv8Attn; rows, tiles_r, ctas and the size of part as planned.
-B200_API int b200_kv8_attention(const Kv8Attn* a, void* stream) {
-  const Kv8Attn& p = *a;
+// a: sizes and cache of the call (rows, tiles_r, ctas and the size of part as planned); the tensors of this call apart from it.
+B200_API int b200_kv8_attention(const Kv8Attn* a, const void* q, const int* lens, void* out, float* part, void* stream) {
+  Kv8Attn p = *a;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.lens = lens;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.part = part;
   if (p.B <= 0 || p.B > 65535 || p.Hkv <= 0 || p.n <= 0 || p.group <= 0 || p.rows <= 0 || p.rows > 32 || p.tiles_r <= 0 || p.ctas <= 0 ||
       p.log2_block < 4 || p.log2_block > 7 || p.most <= 0 || p.most > p.cap || !p.part)
     return -1;
   if (static_cast<long long>(p.rows) * p.tiles_r < static_cast<long long>(p.n) * p.group) return -1;
+  if (static_cast<double>(p.n) * p.group * p.group > 4e9) return -4;
+  p.group_magic = static_cast<uint32_t>((0x100000000ull + p.group - 1) / p.group);
   if ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | p.sb | p.sh) & 15) return -2;
   if (((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.part)) & 15) || ((p.q_sb | p.q_sn | p.q_sh) & 7)) return -2;
   const int nt = (p.rows + 7) / 8;

@@ -35,7 +35,7 @@ class _Attn(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ke", "ve")] + [(n, C.c_longlong) for n in ("sb", "sh", "eb", "eh")] + \
                [(n, C.c_int) for n in ("B", "Hkv", "cap", "D", "log2_block")] + [("q", C.c_void_p)] + \
                [(n, C.c_longlong) for n in ("q_sb", "q_sn", "q_sh")] + [(n, C.c_void_p) for n in ("lens", "out", "part")] + \
-               [(n, C.c_int) for n in ("n", "group", "rows", "tiles_r", "most")] + [("scale_log2", C.c_float), ("ctas", C.c_int)]
+               [(n, C.c_int) for n in ("n", "group", "rows", "tiles_r", "most")] + [("scale_log2", C.c_float), ("ctas", C.c_int), ("group_magic", C.c_uint32)]
 
 
 _fns = None
@@ -50,32 +50,34 @@ def _k():
 
         vp, i, ll = C.c_void_p, C.c_int, C.c_longlong
         _fns = SimpleNamespace(
-            K=K,
+            K=K, check=K._check, stream=K._stream,
             append=K._sig("b200_kv8_append", [C.POINTER(_Cache), vp, vp, C.POINTER(ll), vp, vp, i, vp, vp]),
             rope=K._sig("b200_kv8_rope_append", [C.POINTER(_Cache), vp, ll, i, i, vp, vp, vp, vp, vp, i, vp, vp]),
             decode=K._sig("b200_kv8_decode", [C.POINTER(_Cache), vp, vp, vp, i, i, vp]),
             tiles=K._sig("b200_kv8_tiles", [vp, vp, vp, i, i, i, i, ll, vp]),
             plan=K._sig("b200_kv8_attention_plan", [i] * 5 + [C.POINTER(i)]),
-            attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn), vp]),
+            attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn)] + [vp] * 5),
             long_ok=K._sig("b200_capped_attention_supported", [i, i]),
             long=K._sig("b200_capped_attention", [vp] * 6 + [i] * 12 + [C.c_float] * 3 + [vp, vp]),
         )
     return _fns
 
 
-class _On:
-    """Makes a tensor's device the current one around a launch."""
+_device = torch._C._cuda_getDevice
+_MOST_CALLS = 256       # remembered kinds of calls per cache
 
-    def __init__(self, device):
-        self.guard = None if device.index is None or device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+def _on(device: torch.device):
+    """A guard that makes ``device`` the current one, or None where it is."""
+    return None if device.index == _device() else torch.cuda.device(device)
 
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+
+def _guarded(device: torch.device, fn, *args):
+    guard = _on(device)
+    if guard is None:
+        return fn(*args)
+    with guard:
+        return fn(*args)
 
 
 @dataclass(eq=False)
@@ -110,6 +112,7 @@ class KV8Cache:
         if k.is_cuda and ((k.data_ptr() | v.data_ptr() | k.stride(0) | k.stride(1)) & 15):
             raise ValueError("heads start on 16-byte boundaries")
         self.device = k.device
+        self._calls: dict = {}          # what a kind of call (shapes, pitches, types, numbers) needs: checked once, then looked up
         self._c = _Cache(k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), k.stride(0), k.stride(1), ke.stride(0), ke.stride(1),
                          *k.shape, self.block.bit_length() - 1)
 
@@ -128,15 +131,26 @@ class KV8Cache:
             return tuple(ref.kv8_decode(c, e).transpose(1, 2).to(BF16) for c, e in ((self.k, self.k_exp), (self.v, self.v_exp)))
         k, v = (torch.empty(self.batch, self.capacity, self.kv_heads, self.dim, dtype=BF16, device=self.device) for _ in range(2))
         f = _k()
-        with _On(self.device):
-            f.K._check(f.decode(C.byref(self._c), 0, k.data_ptr(), v.data_ptr(), self.capacity, self.capacity, f.K._stream()), "kv8_decode")
+        _guarded(self.device, lambda: f.K._check(f.decode(C.byref(self._c), 0, k.data_ptr(), v.data_ptr(), self.capacity, self.capacity, f.K._stream()),
+                                                 "kv8_decode"))
         return k, v
 
+    def _call(self, key: tuple, make, *args):
+        call = self._calls.get(key)
+        if call is None:
+            if len(self._calls) >= _MOST_CALLS:
+                self._calls.clear()
+            call = self._calls[key] = make(self, *args)
+        return call
 
-def _index(t: torch.Tensor, cache: KV8Cache, what: str) -> torch.Tensor:
+
+def _index(t: torch.Tensor, cache: KV8Cache, what: str) -> None:
     if t.dtype != torch.int32 or t.shape != (cache.batch,) or t.device != cache.device or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 tensor [{cache.batch}] on the cache's device")
-    return t
+
+
+def _kind(t: torch.Tensor) -> tuple:
+    return t.shape, t.stride(), t.dtype, t.device
 
 
 def _pitch(x: torch.Tensor) -> list:
@@ -144,16 +158,19 @@ def _pitch(x: torch.Tensor) -> list:
     return [0 if n == 1 else st for n, st in zip(x.shape[:-1], x.stride())]
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x, copied unless its head vectors are contiguous and start on 16-byte boundaries."""
-    if x.stride(-1) == 1 and not (x.data_ptr() & 15) and not any(s & 7 for s in _pitch(x)):
-        return x
+def _aligned(x: torch.Tensor) -> bool:
+    """Whether contiguous head vectors start on 16-byte boundaries, apart from the tensor's address."""
+    return x.stride(-1) == 1 and not any(s & 7 for s in _pitch(x))
+
+
+def _copy(x: torch.Tensor) -> torch.Tensor:
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
-    """Write keys and values [B, n, kv_heads, dim] (bf16, any pitches) of positions ``start[b] .. start[b] + n - 1`` into the cache;
-    ``counts``: only the first ``counts[b]`` of a sequence's n."""
+# ------------------------------------------------------------------------------------------
+# append
+# ------------------------------------------------------------------------------------------
+def _append_call(cache, k, v, start, counts):
     if k.dim() != 4 or k.dtype != BF16 or v.dtype != BF16 or k.shape != v.shape or k.device != cache.device or v.device != cache.device:
         raise ValueError("keys and values are bf16 [B, n, kv_heads, dim] on the cache's device")
     B, n, H, D = k.shape
@@ -162,24 +179,36 @@ def append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tenso
     _index(start, cache, "start")
     if counts is not None:
         _index(counts, cache, "counts")
+    if not cache.k.is_cuda or n == 0:
+        return n, False, None, None, 0
+    ok = _aligned(k) and _aligned(v)
+    return n, ok, C.byref(cache._c), (C.c_longlong * 6)(*_pitch(k), *_pitch(v)) if ok else None, _k().K.err_word(cache.device).data_ptr()
+
+
+def append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
+    """Write keys and values [B, n, kv_heads, dim] (bf16, any pitches) of positions ``start[b] .. start[b] + n - 1`` into the cache;
+    ``counts``: only the first ``counts[b]`` of a sequence's n."""
+    n, ok, c, pitch, err = cache._call(("append", _kind(k), _kind(v), _kind(start), None if counts is None else _kind(counts)), _append_call, k, v, start,
+                                    counts)
     if n == 0:
         return
-    if not k.is_cuda:
+    if err == 0:
         return ref.kv8_append(cache, k, v, start, counts)
-    f = _k()
-    k, v = _rows(k), _rows(v)
-    pitch = (C.c_longlong * 6)(*_pitch(k), *_pitch(v))
-    with _On(cache.device):
-        f.K._check(f.append(C.byref(cache._c), k.data_ptr(), v.data_ptr(), pitch, start.data_ptr(), f.K._ptr(counts), n,
-                            f.K.err_word(cache.device).data_ptr(), f.K._stream()), "kv8_append")
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if not ok or (kp | vp) & 15:
+        return append(cache, _copy(k), _copy(v), start, counts)
+    f, cp = _fns, 0 if counts is None else counts.data_ptr()
+    if cache.device.index == _device():
+        f.check(f.append(c, kp, vp, pitch, start.data_ptr(), cp, n, err, f.stream()), "kv8_append")
+    else:
+        with torch.cuda.device(cache.device):
+            f.check(f.append(c, kp, vp, pitch, start.data_ptr(), cp, n, err, f.stream()), "kv8_append")
 
 
-def rope_append(cache: KV8Cache, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, heads: int,
-                bias: Optional[torch.Tensor] = None, clear: bool = False) -> torch.Tensor:
-    """The new token of every sequence: ``qkv`` [B, (heads + 2 kv_heads) dim] (bf16 or fp32) holds its packed projection.  Adds the fp32
-    ``bias`` [(heads + kv_heads) dim] to q and k, turns their neighbouring pairs by the angles of position ``pos[b]`` (``cos`` / ``sin``: fp32
-    [>= capacity, dim / 2]), writes k and v into the cache and returns q as bf16 [B, heads, dim].  Rows whose position lies outside the
-    cache keep an undefined q.  ``clear`` hands an fp32 ``qkv`` back zeroed (the accumulator of a decode step's product)."""
+# ------------------------------------------------------------------------------------------
+# rotate and append
+# ------------------------------------------------------------------------------------------
+def _rope_call(cache, qkv, cos, sin, pos, heads, bias, clear):
     B, D, Hkv = cache.batch, cache.dim, cache.kv_heads
     W = (heads + 2 * Hkv) * D
     if heads <= 0 or heads % Hkv:
@@ -194,30 +223,41 @@ def rope_append(cache: KV8Cache, qkv: torch.Tensor, cos: torch.Tensor, sin: torc
     if clear and qkv.dtype != F32:
         raise ValueError("only an fp32 accumulator is handed back zeroed")
     _index(pos, cache, "pos")
-    if not qkv.is_cuda:
+    ld = 0 if B == 1 else qkv.stride(0)
+    err = _k().K.err_word(cache.device).data_ptr() if cache.k.is_cuda else 0
+    return torch.empty(B, heads, D, dtype=BF16, device=cache.device), C.byref(cache._c), ld, int(qkv.dtype == F32), not (ld * qkv.element_size() & 15), err
+
+
+def rope_append(cache: KV8Cache, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, heads: int,
+                bias: Optional[torch.Tensor] = None, clear: bool = False) -> torch.Tensor:
+    """The new token of every sequence: ``qkv`` [B, (heads + 2 kv_heads) dim] (bf16 or fp32) holds its packed projection.  Adds the fp32
+    ``bias`` [(heads + kv_heads) dim] to q and k, turns their neighbouring pairs by the angles of position ``pos[b]`` (``cos`` / ``sin``: fp32
+    [>= capacity, dim / 2]), writes k and v into the cache and returns q as bf16 [B, heads, dim].  Rows whose position lies outside the
+    cache keep an undefined q.  ``clear`` hands an fp32 ``qkv`` back zeroed (the accumulator of a decode step's product)."""
+    like, c, ld, f32, ok, err = cache._call(("rope", _kind(qkv), _kind(cos), _kind(sin), _kind(pos), heads, None if bias is None else _kind(bias), clear), _rope_call,
+                                          qkv, cos, sin, pos, heads, bias, clear)
+    if err == 0:
         return ref.kv8_rope_append(cache, qkv, cos, sin, pos, heads, bias, clear)
-    f = _k()
-    if (qkv.data_ptr() & 15) or (qkv.stride(0) * qkv.element_size() & 15):
+    x, cp, sp = qkv.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    if not ok or x & 15:
         if clear:
             raise ValueError("an accumulator that is cleared has rows on 16-byte boundaries")
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
-    if (cos.data_ptr() | sin.data_ptr()) & 15:
-        cos, sin = cos.clone(), sin.clone()
-    q = torch.empty(B, heads, D, dtype=BF16, device=cache.device)
-    with _On(cache.device):
-        f.K._check(f.rope(C.byref(cache._c), qkv.data_ptr(), qkv.stride(0), qkv.dtype == F32, clear, f.K._ptr(bias), cos.data_ptr(), sin.data_ptr(),
-                          pos.data_ptr(), q.data_ptr(), heads, f.K.err_word(cache.device).data_ptr(), f.K._stream()), "kv8_rope_append")
+        return rope_append(cache, _copy(qkv), cos, sin, pos, heads, bias)
+    if (cp | sp) & 15:
+        return rope_append(cache, qkv, cos.clone(), sin.clone(), pos, heads, bias, clear)
+    f, q, bp = _fns, torch.empty_like(like), 0 if bias is None else bias.data_ptr()
+    if cache.device.index == _device():
+        f.check(f.rope(c, x, ld, f32, clear, bp, cp, sp, pos.data_ptr(), q.data_ptr(), heads, err, f.stream()), "kv8_rope_append")
+    else:
+        with torch.cuda.device(cache.device):
+            f.check(f.rope(c, x, ld, f32, clear, bp, cp, sp, pos.data_ptr(), q.data_ptr(), heads, err, f.stream()), "kv8_rope_append")
     return q
 
 
-_plans: dict = {}
-
-
-def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optional[float] = None, max_len: Optional[int] = None) -> torch.Tensor:
-    """Causal attention of each sequence's n newest tokens: ``q`` [B, n, heads, dim] (bf16), the last one sees the first ``lens[b]`` positions
-    of the cache, the one before it one fewer, and so on; one that sees nothing gets zeros.  Returns bf16 [B, n, heads, dim].
-    ``scale``: factor of the scores, dim ** -0.5 by default.  ``max_len``: no length is larger (longer ones are cut); the capacity by
-    default.  A smaller bound makes short calls cheaper."""
+# ------------------------------------------------------------------------------------------
+# attention
+# ------------------------------------------------------------------------------------------
+def _attention_call(cache, q, lens, scale, max_len):
     if q.dim() != 4 or q.dtype != BF16 or q.device != cache.device:
         raise ValueError("q is bf16 [B, n, heads, dim] on the cache's device")
     B, n, H, D = q.shape
@@ -229,31 +269,48 @@ def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optio
         raise ValueError(f"max_len lies in 1 .. {cache.capacity}")
     scale = D ** -0.5 if scale is None else float(scale)
     if n == 0:
-        return torch.empty_like(q)
-    if not q.is_cuda:
-        return ref.kv8_attention(q, cache, lens, scale, most)
+        return lambda cache, q, lens: torch.empty_like(q)
+    if not cache.k.is_cuda:
+        return lambda cache, q, lens: ref.kv8_attention(q, cache, lens, scale, most)
     group = H // cache.kv_heads
-    q = _rows(q)
     if n * group > STREAM_ROWS and scale > 0:
-        return _long(q, cache, lens, scale, most)
-    f = _k()
-    out = torch.empty(B, n, H, D, dtype=BF16, device=cache.device)
-    with _On(cache.device):
-        key = (cache.device.index, B, cache.kv_heads, D, n * group, most)
-        plan = _plans.get(key)
-        if plan is None:
-            buf = (C.c_int * 4)()
-            rc = f.plan(B, cache.kv_heads, D, n * group, most, buf)
-            if rc:
-                raise RuntimeError(f"kv8_attention_plan failed with code {rc}")
-            plan = _plans[key] = tuple(buf)
-        rows, tiles_r, ctas, scratch = plan
-        part = torch.empty(scratch, dtype=F32, device=cache.device)
-        c = cache._c
-        p = _Attn(c.k, c.v, c.ke, c.ve, c.sb, c.sh, c.eb, c.eh, B, c.Hkv, c.cap, D, c.log2_block, q.data_ptr(), *_pitch(q), lens.data_ptr(),
-                  out.data_ptr(), part.data_ptr(), n, group, rows, tiles_r, most, scale * 1.4426950408889634, ctas)
-        f.K._check(f.attn(C.byref(p), f.K._stream()), "kv8_attention")
-    return out
+        return lambda cache, q, lens: _long(q, cache, lens, scale, most)
+    ok = _aligned(q)
+    f, c, device = _k(), cache._c, cache.device
+    plan = (C.c_int * 4)()
+    rc = _guarded(device, lambda: f.plan(B, cache.kv_heads, D, n * group, most, plan))
+    if rc:
+        raise RuntimeError(f"kv8_attention_plan failed with code {rc}")
+    rows, tiles_r, ctas, scratch = plan
+    p = _Attn(c.k, c.v, c.ke, c.ve, c.sb, c.sh, c.eb, c.eh, B, c.Hkv, c.cap, D, c.log2_block, 0, *(_pitch(q) if ok else (0, 0, 0)), 0, 0, 0, n, group, rows,
+              tiles_r, most, scale * 1.4426950408889634, ctas)
+    ref_p, check, attn, stream, empty_like = C.byref(p), f.check, f.attn, f.stream, torch.empty_like
+    out_like, part_like = (torch.empty(1, dtype=t, device=device).expand(n) for t, n in ((BF16, q.shape), (F32, (scratch,))))
+
+    def run(cache, q, lens):            # holds no reference to the cache, which holds this
+        qp = q.data_ptr()
+        if not ok or qp & 15:
+            return attention(_copy(q), cache, lens, scale, most)
+        out, part = empty_like(out_like, memory_format=torch.contiguous_format), empty_like(part_like, memory_format=torch.contiguous_format)
+        if device.index == _device():
+            check(attn(ref_p, qp, lens.data_ptr(), out.data_ptr(), part.data_ptr(), stream()), "kv8_attention")
+        else:
+            with torch.cuda.device(device):
+                check(attn(ref_p, qp, lens.data_ptr(), out.data_ptr(), part.data_ptr(), stream()), "kv8_attention")
+        return out
+
+    run.keep = p
+    return run
+
+
+def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optional[float] = None, max_len: Optional[int] = None) -> torch.Tensor:
+    """Causal attention of each sequence's n newest tokens: ``q`` [B, n, heads, dim] (bf16), the last one sees the first ``lens[b]`` positions
+    of the cache, the one before it one fewer, and so on; one that sees nothing gets zeros.  Returns bf16 [B, n, heads, dim].
+    ``scale``: factor of the scores, dim ** -0.5 by default.  ``max_len``: no length is larger (longer ones are cut); the capacity by
+    default.  A smaller bound makes short calls cheaper."""
+    if scale is not None:
+        scale = float(scale)
+    return cache._call((_kind(q), _kind(lens), scale, max_len), _attention_call, q, lens, scale, max_len)(cache, q, lens)
 
 
 def _long(q, cache, lens, scale, most) -> torch.Tensor:
@@ -262,11 +319,13 @@ def _long(q, cache, lens, scale, most) -> torch.Tensor:
     B, n, H, D = q.shape
     Hkv, W = cache.kv_heads, cache.kv_heads * D
     L = (most + 127) // 128 * 128
-    q = q if q.is_contiguous() else q.contiguous()
+    if not q.is_contiguous() or q.data_ptr() & 15:
+        q = _copy(q)
     per = (n + 255) // 256
     if B * per > 65535 or B * max(L, n) >= 2 ** 31:
         raise ValueError(f"{B} sequences of {n} tokens and {most} keys are too many for one call")
-    with _On(cache.device):
+
+    def run():
         K, st = f.K, f.K._stream()
         out = torch.empty(B, n, H, D, dtype=BF16, device=cache.device)
         kv = torch.empty(2, B * L, W, dtype=BF16, device=cache.device)
@@ -275,4 +334,6 @@ def _long(q, cache, lens, scale, most) -> torch.Tensor:
         K._check(f.tiles(lens.data_ptr(), tiles.data_ptr(), out.data_ptr(), B, n, most, L, H * D, st), "kv8_tiles")
         K._check(f.long(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), 0, B * per, B * n, B * L, H, Hkv, D, D,
                         H * D, W, H * D, 2 ** 30, 0, scale, 0.0, 0.0, st, K.err_word(cache.device).data_ptr()), "capped_attention")
-    return out
+        return out
+
+    return _guarded(cache.device, run)

@@ -52,6 +52,25 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     ``top_p`` and at least one token, ``min_p`` (0: off) drops what has less than ``min_p`` times the largest probability.  Every setting is a number
     or a tensor with one value per row (fp32, ``top_k`` int32).  A ``temperature`` of 0 picks the largest logit, the lowest index among
     equal ones.  NaN logits count as -inf; a row without any logit above -inf gives -1."""
+    key = (logits.shape, logits.stride(), logits.dtype, logits.device, uniform.shape, uniform.stride(), uniform.dtype, uniform.device,
+           *(_kind(x) for x in (temperature, top_k, top_p, min_p)))
+    call = _calls.get(key)
+    if call is None:
+        if len(_calls) >= 256:
+            _calls.clear()
+        call = _calls[key] = _checked(logits, uniform, temperature, top_k, top_p, min_p)
+    return call(logits, uniform, temperature, top_k, top_p, min_p)
+
+
+_calls: dict = {}       # kinds of calls (shapes, pitches, types, numbers), checked once
+
+
+def _kind(x):
+    return (x.shape, x.stride(), x.dtype, x.device) if torch.is_tensor(x) else x
+
+
+def _checked(logits, uniform, temperature, top_k, top_p, min_p):
+    """Checks a kind of call and returns the function that makes it."""
     if logits.dim() != 2 or logits.dtype not in (BF16, F32) or logits.shape[1] == 0 or logits.stride(1) != 1:
         raise ValueError("logits are bf16 or fp32 [B, vocab] with contiguous rows")
     B, V = logits.shape
@@ -66,16 +85,25 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     p, p0 = _setting(top_p, "top_p", logits, F32, 0, 1)
     m, m0 = _setting(min_p, "min_p", logits, F32, 0, 1)
     k, k0 = _setting(top_k, "top_k", logits, torch.int32, 0, 2 ** 31 - 1)
+    device = logits.device
     if B == 0:
-        return torch.empty(0, dtype=torch.int64, device=logits.device)
+        return lambda *a: torch.empty(0, dtype=torch.int64, device=device)
     if not logits.is_cuda:
-        return ref.sample_tokens(logits, uniform, t0 if t is None else t, k0 if k is None else k, p0 if p is None else p, m0 if m is None else m)
-    from .kv8 import _On
-
+        return lambda x, u, t, k, p, m: ref.sample_tokens(x, u, *(0 if a is None else a for a in (t, k, p, m)))
     K, fn = _k()
-    out = torch.empty(B, dtype=torch.int64, device=logits.device)
-    a = _Sample(logits.data_ptr(), max(logits.stride(0), V), V, 0, uniform.data_ptr(), K._ptr(t), K._ptr(p), K._ptr(m), K._ptr(k), t0, p0, m0, int(k0),
-                out.data_ptr())
-    with _On(logits.device):
-        K._check(fn(C.byref(a), B, logits.dtype == BF16, K._stream()), "sample")
-    return out
+    ld, is_bf16, k0 = max(logits.stride(0), V), logits.dtype == BF16, int(k0)
+    check, stream, current, byref = K._check, K._stream, torch._C._cuda_getDevice, C.byref
+    like = torch.empty(B, dtype=torch.int64, device=device)
+    ptr = lambda given, x: 0 if given is None else x.data_ptr()  # noqa: E731
+
+    def run(x, u, temperature, top_k, top_p, min_p):
+        out = torch.empty_like(like)
+        a = _Sample(x.data_ptr(), ld, V, 0, u.data_ptr(), ptr(t, temperature), ptr(p, top_p), ptr(m, min_p), ptr(k, top_k), t0, p0, m0, k0, out.data_ptr())
+        if device.index == current():
+            check(fn(byref(a), B, is_bf16, stream()), "sample")
+        else:
+            with torch.cuda.device(device):
+                check(fn(byref(a), B, is_bf16, stream()), "sample")
+        return out
+
+    return run
