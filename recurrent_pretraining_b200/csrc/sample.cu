@@ -4,13 +4,15 @@
 //     top-k keeps what is not below the k-th value, top-p the longest prefix with sum(w) <= p sum(all w) (at least one token),
 //     min-p what has w_i >= m;  the token is the first index, in the vocabulary's order, with sum_{kept, j <= i} w_j > u sum_kept w.
 //
-// A row belongs to a cluster of up to eight CTAs, each with a contiguous slice of the logits in shared memory: they are read from
+// A row belongs to a cluster of up to sixteen CTAs, each with a contiguous slice of the logits in shared memory: they are read from
 // global memory once.  Weights are 44-bit fixed-point numbers formed in double precision (2^-44 of the largest), so sums are
 // integers: exact in any order, equal from run to run, and a prefix ends where its definition says.  All filters are one cut (key, index)
-// in the descending order.  It is found by a histogram over 1/16 octave of weight (counts for k, sums for p), whose
-// bins the CTAs add up through distributed shared memory; the candidates of the one bin that the cut falls into are ranked against each
-// other.  Should they be too many (equal logits), the bin is divided again by the bits of its keys, down to a single value whose ties
-// are counted in index order.
+// in the descending order.  It is found by a histogram over 1/32 octave of weight (counts for k, sums for p), whose
+// bins every CTA adds up through distributed shared memory; the candidates of the one bin that the cut falls into are collected by every CTA
+// and divided further by the bits of their keys until few are left, which are ranked against each other.  Should they be too many to be
+// collected (equal logits), the whole slices are divided again, down to a single value whose ties are counted in index order.
+//
+// A row is bound by the latency of its stages, which the machine runs side by side for a batch: TODO_FIG
 #include <cooperative_groups.h>
 
 #include <utility>
@@ -20,14 +22,15 @@
 namespace b200 {
 namespace cg = cooperative_groups;
 
-constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_BINS = 512, SP_CAND = 1024, SP_MAX_CTAS = 8, SP_TAB = 256;
-constexpr float SP_BINS_PER_OCTAVE = 16.f;
+constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_BINS = 512, SP_CAND = 1024, SP_FEW = 128, SP_MAX_CTAS = 16, SP_TAB = 256, SP_LIST = 512;
+constexpr float SP_BINS_PER_OCTAVE = 32.f;
 constexpr int SP_ONE = 44;                          // a weight of 1 is 2^44; 2^18 of them fit the sums
+static_assert(SP_BINS == SP_THREADS, "a bin per thread");
 
 struct SampleParams {
   const void* logits;                               // [B, V], row pitch ld
   long long ld;
-  int V, per;                                       // per: slice of a CTA, a multiple of 8
+  int V, per;                                       // per: slice of a CTA, a multiple of SP_THREADS
   const float* uniform;
   const float *temperature, *top_p, *min_p;         // [B]; null: the value below
   const int* top_k;
@@ -36,20 +39,30 @@ struct SampleParams {
   long long* out;
 };
 
+struct SampleHist {
+  uint32_t cnt[SP_BINS], lo[SP_BINS], hi[SP_BINS];  // sums of weights as two words
+};
 struct SampleShared {
   union {
-    struct { uint32_t cnt[SP_BINS], lo[SP_BINS], hi[SP_BINS]; } h;             // this slice
-    struct { uint32_t key[SP_CAND], idx[SP_CAND]; } c;
-  } a;
+    SampleHist hist;                                // this slice
+    struct { uint32_t key[SP_CAND], idx[SP_CAND]; } sel;        // the last few candidates, when all CTAs have read the histogram
+  } h;
+  uint32_t key[SP_CAND], idx[SP_CAND];              // candidates of this slice
   union {
-    struct { uint32_t cnt[SP_BINS]; unsigned long long mass[SP_BINS]; } h;     // the whole row
-    unsigned long long sorted[SP_CAND];
-  } b;
+    struct {
+      uint32_t key[SP_CAND], idx[SP_CAND];          // of the row
+      union {
+        SampleHist sub;
+        unsigned long long sorted[SP_CAND];
+      } u;
+    } all;
+    uint16_t list[SP_WARPS][SP_LIST];               // kept elements of a warp's part, in order
+  } w;
   double tab[SP_TAB];                               // 2^(44 - i / 256)
   unsigned long long red[SP_WARPS], red2[SP_WARPS];
   unsigned long long xch[2][SP_MAX_CTAS];           // what the CTAs of the cluster tell each other
   uint32_t xa[2][SP_MAX_CTAS], xb[2][SP_MAX_CTAS];
-  uint32_t ncand;
+  uint32_t ncand, nsel, order[SP_FEW];
   int found, found2;
   unsigned long long before[2];
 };
@@ -74,21 +87,48 @@ __device__ __forceinline__ unsigned long long warp_scan64(unsigned long long v) 
   return v;
 }
 
+// w to a bin of a histogram; the carry of the lower word goes to the upper one, so the sum is exact whatever the order.
+__device__ __forceinline__ void sp_add(SampleHist& h, int bin, unsigned long long w) {
+  const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&h.lo[bin], l);
+  const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + l < old ? 1u : 0u);
+  if (up) atomicAdd(&h.hi[bin], up);
+}
+
+struct SampleScale {
+  float mx, cf;
+  double c, mxc;                                    // log2(e) / T; max times that
+};
+// 2^-y, y = (max - v) log2(e) / T = a + i / 256 + r, in units of 2^-44.  Not inlined: a row runs through every stage of the kernel once,
+// and with eight copies of this in it the fetching of instructions took a third of its time.
+__device__ __noinline__ unsigned long long sp_weight(float v, float mx, float cf, double c, double mxc, const double* tab) {
+  const double y = fma(-static_cast<double>(v), c, mxc);
+  const double big = 6755399441055744.0 / SP_TAB;   // 1.5 * 2^52 / 256: adding it leaves round(256 y) in the low bits
+  const double z = y + big;
+  const int q = __double2loint(z);
+  const double r = y - (z - big);                   // |r| <= 2^-9; 2^-r = 1 - z + z^2 / 2 - z^3 / 6, z = r ln 2, to 2e-13
+  const double e = fma(r, fma(r, fma(r, -0.055504108664821580, 0.24022650695910071), -0.69314718055994531), 1.0);
+  const double f = fma(tab[q & (SP_TAB - 1)], e, 4503599627370496.0);           // 2^52: the low bits are the rounded integer
+  const unsigned long long w = (static_cast<unsigned long long>(__double_as_longlong(f)) & 0xFFFFFFFFFFFFFull) >> (q / SP_TAB & 63);
+  return v == mx ? 1ull << SP_ONE : (mx - v) * cf < SP_ONE + 1.f ? w : 0ull;    // (infinities, too)
+}
+
 template <typename T>
-__global__ void __launch_bounds__(SP_THREADS)
+__global__ void __launch_bounds__(SP_THREADS, 2)
 sample_kernel(const SampleParams p) {
-  extern __shared__ float sx[];                     // [per] logits of the slice, NaN as -inf
+  extern __shared__ float sx[];                     // logits of the slice, NaN as -inf; element i at i + i / 32
   __shared__ SampleShared s;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lo = rank * p.per, n = max(0, min(p.per, p.V - lo));
-  const int chunk = p.per / SP_WARPS;               // warps own contiguous parts of the slice
+  const int chunk = p.per / SP_WARPS, each = chunk / 32;        // warps own contiguous parts of the slice, lanes parts of those
   const int w0 = min(n, warp * chunk), w1 = min(n, w0 + chunk);
   int phase = 0;                                    // exchanges alternate between two places
+  auto at = [&](int i) -> float& { return sx[i + (i >> 5)]; };  // both orders of access meet no bank twice
 
   auto started = cluster.barrier_arrive();          // before the first access to another CTA's memory it has to be running
   if (tid < SP_TAB) s.tab[tid] = exp2(static_cast<double>(SP_ONE) - tid / static_cast<double>(SP_TAB));
+  s.h.hist.cnt[tid] = s.h.hist.lo[tid] = s.h.hist.hi[tid] = 0;
   pdl_trigger();
   pdl_wait();
   const T* x = static_cast<const T*>(p.logits) + static_cast<long long>(row) * p.ld + lo;
@@ -98,50 +138,37 @@ sample_kernel(const SampleParams p) {
   const float u = p.uniform[row];
 
   // ---- the slice, its maximum and where it is first
-  uint32_t best = 0, at = 0;
+  uint32_t best = 0, where = 0;
   auto take = [&](int i, float v) {
     v = v == v ? v + 0.f : -INFINITY;               // -0 and 0 are one value
-    sx[i] = v;
+    at(i) = v;
     const uint32_t k = sp_key(v);
-    if (k > best) { best = k; at = lo + i; }        // a thread meets its elements in index order
+    if (k > best) { best = k; where = lo + i; }     // a thread meets its elements in index order
   };
-  constexpr int VEC = 16 / sizeof(T);
-  if (!((reinterpret_cast<uintptr_t>(x)) & 15)) {
-    const int nv = n / VEC;
+  if (sizeof(T) == 2 && !(reinterpret_cast<uintptr_t>(x) & 3)) {
 #pragma unroll 4
-    for (int i = tid; i < nv; i += SP_THREADS) {
-      const uint4 r = __ldg(reinterpret_cast<const uint4*>(x) + i);
-      if constexpr (sizeof(T) == 4) {
-        take(4 * i, __uint_as_float(r.x)); take(4 * i + 1, __uint_as_float(r.y)); take(4 * i + 2, __uint_as_float(r.z)); take(4 * i + 3, __uint_as_float(r.w));
-      } else {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack_bf16x2(w[j]);
-          take(8 * i + 2 * j, f.x);
-          take(8 * i + 2 * j + 1, f.y);
-        }
-      }
+    for (int i = tid; i < n / 2; i += SP_THREADS) {
+      const float2 f = unpack_bf16x2(__ldg(reinterpret_cast<const uint32_t*>(x) + i));
+      take(2 * i, f.x);
+      take(2 * i + 1, f.y);
     }
-    for (int i = nv * VEC + tid; i < n; i += SP_THREADS) take(i, static_cast<float>(x[i]));
+    if ((n & 1) && tid == 0) take(n - 1, static_cast<float>(x[n - 1]));
   } else {
 #pragma unroll 8
     for (int i = tid; i < n; i += SP_THREADS) take(i, static_cast<float>(x[i]));
   }
   // larger key first, then the lower index
-  unsigned long long top = (static_cast<unsigned long long>(best) << 32) | (0xFFFFFFFFu - at);
+  unsigned long long top = (static_cast<unsigned long long>(best) << 32) | (0xFFFFFFFFu - where);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s.red[warp] = top;
   __syncthreads();
+  cluster.barrier_wait(std::move(started));
   if (warp == 0) {
     top = lane < SP_WARPS ? s.red[lane] : 0ull;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     top = __shfl_sync(0xffffffffu, top, 0);
-  }
-  cluster.barrier_wait(std::move(started));
-  if (warp == 0) {
     if (lane < C) cluster.map_shared_rank(&s, lane)->xch[phase][rank] = top;
   }
   cluster.sync();
@@ -155,22 +182,13 @@ sample_kernel(const SampleParams p) {
     return;                                         // no CTA touches another's memory after the barrier
   }
 
-  // ---- weights: 2^-y with y = (max - x) log2(e) / T = a + i / 256 + r
-  const double c = 1.4426950408889634 / static_cast<double>(T_), mxd = mx;
-  const float cf = static_cast<float>(c);
-  auto weight = [&](float v) -> unsigned long long {
-    if (v == mx) return 1ull << SP_ONE;
-    const float yf = (mx - v) * cf;
-    if (!(yf < SP_ONE + 1.f)) return 0ull;
-    const double y = (mxd - static_cast<double>(v)) * c;
-    const double big = 6755399441055744.0 / SP_TAB; // 1.5 * 2^52 / 256: adding it leaves round(256 y) in the low bits
-    const double z = y + big;
-    const int q = __double2loint(z);
-    const double r = y - (z - big);                 // |r| <= 2^-9; 2^-r = 1 - z + z^2 / 2 - z^3 / 6, z = r ln 2, to 2e-13
-    const double e = fma(r, fma(r, fma(r, -0.055504108664821580, 0.24022650695910071), -0.69314718055994531), 1.0);
-    const double f = fma(s.tab[q & (SP_TAB - 1)], e, 4503599627370496.0);       // 2^52: the low bits are the rounded integer
-    return (static_cast<unsigned long long>(__double_as_longlong(f)) & 0xFFFFFFFFFFFFFull) >> (q / SP_TAB);
-  };
+  SampleScale sc;
+  sc.mx = mx;
+  sc.c = 1.4426950408889634 / static_cast<double>(T_);
+  sc.cf = static_cast<float>(sc.c);
+  sc.mxc = static_cast<double>(mx) * sc.c;
+  const float cf = sc.cf;
+  auto weight = [&](float v) { return sp_weight(v, sc.mx, sc.cf, sc.c, sc.mxc, s.tab); };
 
   // ---- the cut: kept are keys above cut_key, and those equal to it with an index up to cut_idx
   uint32_t cut_key = 0;
@@ -179,16 +197,46 @@ sample_kernel(const SampleParams p) {
     if (key > cut_key || (key == cut_key && idx < cut_idx)) { cut_key = key; cut_idx = idx; }
   };
   if (min_p > 0.f) {
-    const double thr = mxd + static_cast<double>(T_) * log(static_cast<double>(min_p));
+    const double thr = static_cast<double>(mx) + static_cast<double>(T_) * log(static_cast<double>(min_p));
     float f = static_cast<float>(thr);
     uint32_t k = sp_key(f + 0.f);
     if (static_cast<double>(f) < thr) ++k;          // the least float that is not below
     cut(k, INT_MAX);
   }
   bool by_k = top_k > 0 && top_k < p.V, by_p = top_p > 0.f && top_p < 1.f;
+  unsigned long long limit = 0, mass_before = 0, cnt_before = 0;    // largest prefix sum; what lies in front of the present subset
+
+  // The first bin in which a limit is passed (SP_BINS: none), from the counts and sums of thread's bin; moves the sums in front along.
+  auto crossing = [&](uint32_t cnt_b, unsigned long long mass_b, bool first) -> int {
+    unsigned long long cs = by_k ? warp_scan64(cnt_b) : 0ull, ms = by_p ? warp_scan64(mass_b) : 0ull;
+    if (lane == 31) { s.red[warp] = cs; s.red2[warp] = ms; }
+    if (tid == 0) { s.found = SP_BINS; s.found2 = SP_BINS; s.nsel = 0; }
+    __syncthreads();
+    unsigned long long total = 0;
+    for (int w = 0; w < SP_WARPS; ++w) {
+      if (w < warp) { cs += s.red[w]; ms += s.red2[w]; }
+      total += s.red2[w];
+    }
+    cs += cnt_before;
+    ms += mass_before;
+    if (first) limit = static_cast<unsigned long long>(static_cast<double>(top_p) * static_cast<double>(total));
+    const bool past_k = by_k && cs >= static_cast<unsigned long long>(top_k), past_p = by_p && ms > limit;
+    const uint32_t vk = __ballot_sync(0xffffffffu, past_k), vp = __ballot_sync(0xffffffffu, past_p);
+    if (lane == 0 && vk) atomicMin(&s.found, 32 * warp + __ffs(vk) - 1);
+    if (lane == 0 && vp) atomicMin(&s.found2, 32 * warp + __ffs(vp) - 1);
+    __syncthreads();
+    const int bk = s.found, bp = s.found2, hit = min(bk, bp);
+    if (hit == SP_BINS) return hit;
+    by_k = by_k && bk == hit;
+    by_p = by_p && bp == hit;
+    if (tid == hit) { s.before[0] = cs - cnt_b; s.before[1] = ms - mass_b; }
+    __syncthreads();
+    cnt_before = s.before[0];
+    mass_before = s.before[1];
+    return hit;
+  };
+
   if (by_k || by_p) {
-    unsigned long long limit = 0, mass_before = 0;  // largest prefix sum; what lies in front of the present subset
-    unsigned long long cnt_before = 0;
     const float bin_scale = cf * SP_BINS_PER_OCTAVE;
     bool first = true;
     uint32_t kmin = 0, kmax = 0xFFFFFFFFu;
@@ -199,109 +247,150 @@ sample_kernel(const SampleParams p) {
       return k < kmin || k > kmax ? -1 : static_cast<int>((kmax - k) >> shift);
     };
     while (true) {
-      for (int i = tid; i < SP_BINS; i += SP_THREADS) s.a.h.cnt[i] = s.a.h.lo[i] = s.a.h.hi[i] = 0;
-      __syncthreads();
+      // most tokens of a vocabulary are improbable and share the last bin: they are added up in registers
+      uint32_t rest = 0;
+      unsigned long long rest_w = 0;
+#pragma unroll 2
       for (int i = w0 + lane; i < w1; i += 32) {
-        const float v = sx[i];
-        const int b = bin_of(v);
-        if (b < 0) continue;
-        atomicAdd(&s.a.h.cnt[b], 1u);
-        if (by_p) {
-          const unsigned long long w = weight(v);
-          const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&s.a.h.lo[b], l);
-          const uint32_t hi = static_cast<uint32_t>(w >> 32) + (old + l < old ? 1u : 0u);
-          if (hi) atomicAdd(&s.a.h.hi[b], hi);
+        const float v = at(i);
+        const int bin = bin_of(v);
+        const unsigned long long w = by_p ? weight(v) : 0ull;
+        if (bin == SP_BINS - 1) {
+          ++rest;
+          rest_w += w;
+        } else if (bin >= 0) {
+          if (by_k) atomicAdd(&s.h.hist.cnt[bin], 1u);
+          if (w) sp_add(s.h.hist, bin, w);
         }
       }
+      rest = __reduce_add_sync(0xffffffffu, rest);
+      rest_w = warp_sum64(rest_w);
+      if (lane == 0 && rest) {
+        atomicAdd(&s.h.hist.cnt[SP_BINS - 1], rest);
+        sp_add(s.h.hist, SP_BINS - 1, rest_w);
+      }
+      if (tid == 0) s.ncand = 0;
       cluster.sync();
-      {                                             // each CTA adds up its share of the bins and tells everyone
-        const int share = SP_BINS / C;
-        for (int i = tid; i < share; i += SP_THREADS) {
-          const int b = rank * share + i;
-          uint32_t cnt = 0;
-          unsigned long long mass = 0;
-          for (int q = 0; q < C; ++q) {
-            const SampleShared* r = cluster.map_shared_rank(&s, q);
-            cnt += r->a.h.cnt[b];
-            mass += (static_cast<unsigned long long>(r->a.h.hi[b]) << 32) + r->a.h.lo[b];
-          }
-          for (int q = 0; q < C; ++q) {
-            SampleShared* r = cluster.map_shared_rank(&s, q);
-            r->b.h.cnt[b] = cnt;
-            r->b.h.mass[b] = mass;
-          }
+      uint32_t cnt_b = 0;
+      unsigned long long mass_b = 0;
+#pragma unroll 4
+      for (int q = 0; q < C; ++q) {
+          const SampleHist& h = cluster.map_shared_rank(&s, q)->h.hist;
+          if (by_k) cnt_b += h.cnt[tid];
+          if (by_p) mass_b += (static_cast<unsigned long long>(h.hi[tid]) << 32) + h.lo[tid];
         }
-      }
-      if (tid == 0) { s.found = SP_BINS; s.found2 = SP_BINS; s.ncand = 0; }
-      cluster.sync();
-      // one bin per thread: prefix sums, the first bin in which a limit is passed
-      const uint32_t cnt_b = s.b.h.cnt[tid];
-      const unsigned long long mass_b = s.b.h.mass[tid];
-      unsigned long long cs = warp_scan64(cnt_b), ms = warp_scan64(mass_b);
-      if (lane == 31) { s.red[warp] = cs; s.red2[warp] = ms; }
-      __syncthreads();
-      unsigned long long total = 0;
-      for (int w = 0; w < SP_WARPS; ++w) {
-        if (w < warp) { cs += s.red[w]; ms += s.red2[w]; }
-        total += s.red2[w];
-      }
-      cs += cnt_before;
-      ms += mass_before;
-      if (first) limit = static_cast<unsigned long long>(static_cast<double>(top_p) * static_cast<double>(total));
-      if (by_k && cs >= static_cast<unsigned long long>(top_k)) atomicMin(&s.found, tid);
-      if (by_p && ms > limit) atomicMin(&s.found2, tid);
-      __syncthreads();
-      const int bk = s.found, bp = s.found2, hit = min(bk, bp);
+      const int hit = crossing(cnt_b, mass_b, first);
       if (hit == SP_BINS) break;                    // the rest passes no limit (the same in all CTAs)
-      by_k = by_k && bk == hit;
-      by_p = by_p && bp == hit;
-      if (tid == hit) { s.before[0] = cs - cnt_b; s.before[1] = ms - mass_b; }
-      const uint32_t cand = s.b.h.cnt[hit];
-      __syncthreads();
-      cnt_before = s.before[0];
-      mass_before = s.before[1];
+      // ---- the bin's candidates, as far as they fit
+#pragma unroll 2
+      for (int i = w0 + lane; i < w1; i += 32) {
+        const float v = at(i);
+        if (bin_of(v) == hit) {
+          const uint32_t slot = atomicAdd(&s.ncand, 1u);
+          if (slot < SP_CAND) { s.key[slot] = sp_key(v); s.idx[slot] = lo + i; }
+        }
+      }
+      cluster.sync();
+      // where the slices' candidates end: lane q has that of slice q
+      uint32_t end = lane < C ? cluster.map_shared_rank(&s, lane)->ncand : 0u;
+#pragma unroll
+      for (int o = 1; o < SP_MAX_CTAS; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += up;
+      }
+      const uint32_t cand = __shfl_sync(0xffffffffu, end, SP_MAX_CTAS - 1);
       if (cand <= SP_CAND) {
-        // ---- rank the candidates
-        for (int i = w0 + lane; i < w1; i += 32)
-          if (bin_of(sx[i]) == hit) {
-            const uint32_t at2 = atomicAdd(&s.ncand, 1u);
-            s.a.c.key[at2] = sp_key(sx[i]);
-            s.a.c.idx[at2] = lo + i;
-          }
-        cluster.sync();
-        uint32_t mykey[2], myidx[2];
-        int have = 0;
-        for (int i = tid; i < static_cast<int>(cand); i += SP_THREADS) {        // the i-th of all lists together
-          uint32_t j = i;
+        // ---- all of them in every CTA
+        for (uint32_t i0 = 32 * warp; i0 < cand; i0 += SP_THREADS) {
+          const uint32_t i = i0 + lane;
+          uint32_t from = 0;
           int q = 0;
-          for (; q < C; ++q) {
-            const uint32_t m = cluster.map_shared_rank(&s, q)->ncand;
-            if (j < m) break;
-            j -= m;
+#pragma unroll 1
+          for (int j = 0; j < C - 1; ++j) {
+            const uint32_t e = __shfl_sync(0xffffffffu, end, j);
+            if (i >= e) { q = j + 1; from = e; }
           }
-          const SampleShared* r = cluster.map_shared_rank(&s, q);
-          mykey[have] = r->a.c.key[j];
-          myidx[have++] = r->a.c.idx[j];
-        }
-        cluster.sync();                             // everyone has read the lists: they become one here
-        have = 0;
-        for (int i = tid; i < static_cast<int>(cand); i += SP_THREADS) {
-          s.a.c.key[i] = mykey[have];
-          s.a.c.idx[i] = myidx[have++];
+          if (i < cand) {
+            const SampleShared* r = cluster.map_shared_rank(&s, q);
+            s.w.all.key[i] = r->key[i - from];
+            s.w.all.idx[i] = r->idx[i - from];
+          }
         }
         __syncthreads();
-        for (int i = tid; i < static_cast<int>(cand); i += SP_THREADS) {
-          const uint32_t k = s.a.c.key[i], d = s.a.c.idx[i];
-          int r = 0;
-          for (int j = 0; j < static_cast<int>(cand); ++j) r += s.a.c.key[j] > k || (s.a.c.key[j] == k && s.a.c.idx[j] < d);
-          s.b.sorted[r] = (static_cast<unsigned long long>(k) << 32) | d;
+        // ---- divided by the bits of their keys until few are left
+        kmin = 0;
+        kmax = 0xFFFFFFFFu;
+        uint32_t left = cand;
+        while (left > SP_FEW) {
+          uint32_t a = 0xFFFFFFFFu, z = 0;
+          for (uint32_t i = tid; i < cand; i += SP_THREADS) {
+            const uint32_t k = s.w.all.key[i];
+            if (k >= kmin && k <= kmax) { a = min(a, k); z = max(z, k); }
+          }
+          a = __reduce_min_sync(0xffffffffu, a);
+          z = __reduce_max_sync(0xffffffffu, z);
+          if (lane == 0) { s.red[warp] = a; s.red2[warp] = z; }
+          s.w.all.u.sub.cnt[tid] = s.w.all.u.sub.lo[tid] = s.w.all.u.sub.hi[tid] = 0;
+          __syncthreads();
+          for (int w = 0; w < SP_WARPS; ++w) { a = min(a, static_cast<uint32_t>(s.red[w])); z = max(z, static_cast<uint32_t>(s.red2[w])); }
+          kmin = a;
+          kmax = z;
+          if (kmin == kmax) break;                  // equal logits: ranked by their indices
+          shift = max(0, 32 - __clz(kmax - kmin) - 9);
+          for (uint32_t i = tid; i < cand; i += SP_THREADS) {
+            const uint32_t k = s.w.all.key[i];
+            if (k < kmin || k > kmax) continue;
+            const int bin = static_cast<int>((kmax - k) >> shift);
+            atomicAdd(&s.w.all.u.sub.cnt[bin], 1u);
+            if (by_p) sp_add(s.w.all.u.sub, bin, weight(sp_unkey(k)));
+          }
+          __syncthreads();
+          const uint32_t here = s.w.all.u.sub.cnt[tid];
+          const int sub = crossing(here, (static_cast<unsigned long long>(s.w.all.u.sub.hi[tid]) << 32) + s.w.all.u.sub.lo[tid], false);
+          left = s.w.all.u.sub.cnt[sub];                  // there is one: the bin passes the limit
+          const uint32_t high = kmax - (static_cast<uint32_t>(sub) << shift);
+          kmin = max(kmin, high - ((1u << shift) - 1));
+          kmax = high;
+          __syncthreads();                          // sub has been read
+        }
+        // ---- ranked
+        if (tid == 0) s.nsel = 0;
+        if (tid < SP_FEW) s.order[tid] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < cand; i += SP_THREADS) {
+          const uint32_t k = s.w.all.key[i];
+          if (k >= kmin && k <= kmax) {
+            const uint32_t slot = atomicAdd(&s.nsel, 1u);
+            s.h.sel.key[slot] = k;
+            s.h.sel.idx[slot] = s.w.all.idx[i];
+          }
         }
         __syncthreads();
-        if (by_k) cut(static_cast<uint32_t>(s.b.sorted[top_k - cnt_before - 1] >> 32), INT_MAX);
+        if (left <= SP_FEW) {                       // four threads per candidate
+          constexpr int SEG = SP_THREADS / SP_FEW;
+          const uint32_t i = tid % SP_FEW;
+          if (i < left) {
+            const uint32_t k = s.h.sel.key[i], d = s.h.sel.idx[i];
+            uint32_t r = 0;
+            for (uint32_t j = tid / SP_FEW; j < left; j += SEG) r += s.h.sel.key[j] > k || (s.h.sel.key[j] == k && s.h.sel.idx[j] < d);
+            if (r) atomicAdd(&s.order[i], r);
+          }
+          __syncthreads();
+          if (tid < left) s.w.all.u.sorted[s.order[tid]] = (static_cast<unsigned long long>(s.h.sel.key[tid]) << 32) | s.h.sel.idx[tid];
+        } else {
+          for (uint32_t i = tid; i < left; i += SP_THREADS) {
+            const uint32_t k = s.h.sel.key[i], d = s.h.sel.idx[i];
+            uint32_t r = 0;
+            for (uint32_t j = 0; j < left; ++j) r += s.h.sel.key[j] > k || (s.h.sel.key[j] == k && s.h.sel.idx[j] < d);
+            s.w.all.u.sorted[r] = (static_cast<unsigned long long>(k) << 32) | d;
+          }
+        }
+        __syncthreads();
+        if (by_k) cut(static_cast<uint32_t>(s.w.all.u.sorted[top_k - cnt_before - 1] >> 32), INT_MAX);
         if (by_p) {                                 // two neighbouring candidates per thread
           unsigned long long w[2], run;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < static_cast<int>(cand) ? weight(sp_unkey(static_cast<uint32_t>(s.b.sorted[2 * tid + j] >> 32))) : 0ull;
+          for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < static_cast<int>(left) ? weight(sp_unkey(static_cast<uint32_t>(s.w.all.u.sorted[2 * tid + j] >> 32))) : 0ull;
           run = warp_scan64(w[0] + w[1]);
           if (lane == 31) s.red[warp] = run;
           if (tid == 0) s.found = 0;
@@ -312,23 +401,23 @@ sample_kernel(const SampleParams p) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             run += w[j];
-            if (2 * tid + j < static_cast<int>(cand) && run <= limit) keep = 2 * tid + j + 1;
+            if (2 * tid + j < static_cast<int>(left) && run <= limit) keep = 2 * tid + j + 1;
           }
           if (keep) atomicMax(&s.found, keep);
           __syncthreads();
           keep = s.found;
-          if (keep == 0 && cnt_before == 0) keep = 1;           // the most probable token stays
-          if (keep) cut(static_cast<uint32_t>(s.b.sorted[keep - 1] >> 32), static_cast<int>(static_cast<uint32_t>(s.b.sorted[keep - 1])));
-          else cut(static_cast<uint32_t>(s.b.sorted[0] >> 32), static_cast<int>(static_cast<uint32_t>(s.b.sorted[0])) - 1);
+          const unsigned long long last = s.w.all.u.sorted[max(keep, 1) - 1];
+          if (keep == 0 && mass_before == 0) keep = 1;          // the most probable token stays
+          cut(static_cast<uint32_t>(last >> 32), static_cast<int>(static_cast<uint32_t>(last)) - (keep ? 0 : 1));
         }
         break;
       }
       // ---- too many: divide the bin by the bits of its keys
       uint32_t a = 0xFFFFFFFFu, z = 0;
       for (int i = w0 + lane; i < w1; i += 32)
-        if (bin_of(sx[i]) == hit) {
-          a = min(a, sp_key(sx[i]));
-          z = max(z, sp_key(sx[i]));
+        if (bin_of(at(i)) == hit) {
+          a = min(a, sp_key(at(i)));
+          z = max(z, sp_key(at(i)));
         }
       a = __reduce_min_sync(0xffffffffu, a);
       z = __reduce_max_sync(0xffffffffu, z);
@@ -341,6 +430,7 @@ sample_kernel(const SampleParams p) {
         r->xa[phase][rank] = static_cast<uint32_t>(a2);
         r->xb[phase][rank] = static_cast<uint32_t>(z2);
       }
+      s.h.hist.cnt[tid] = s.h.hist.lo[tid] = s.h.hist.hi[tid] = 0;    // read by all before the barrier in front of the candidates' counts
       cluster.sync();
       kmin = 0xFFFFFFFFu;
       kmax = 0;
@@ -355,11 +445,11 @@ sample_kernel(const SampleParams p) {
       const unsigned long long w = weight(sp_unkey(kmin));
       unsigned long long keep = cand;
       if (by_p && w) keep = limit > mass_before ? min(keep, (limit - mass_before) / w) : 0ull;
-      if (keep == 0 && cnt_before == 0) keep = 1;
+      if (keep == 0 && mass_before == 0) keep = 1;
       cut(kmin, keep == 0 ? -1 : INT_MAX);
       if (keep && keep < cand) {                    // the index of the last one that stays
         uint32_t mine = 0;
-        for (int i = w0 + lane; i < w1; i += 32) mine += sp_key(sx[i]) == kmin;
+        for (int i = w0 + lane; i < w1; i += 32) mine += sp_key(at(i)) == kmin;
         mine = __reduce_add_sync(0xffffffffu, mine);
         if (lane == 0) s.red[warp] = mine;
         __syncthreads();
@@ -375,7 +465,7 @@ sample_kernel(const SampleParams p) {
         for (int q = 0; q < warp; ++q) { here = here && left > s.red[q]; left -= s.red[q]; }
         if (here && left <= mine) {
           for (int i0 = w0; i0 < w1; i0 += 32) {
-            const bool eq = i0 + lane < w1 && sp_key(sx[i0 + lane]) == kmin;
+            const bool eq = i0 + lane < w1 && sp_key(at(i0 + lane)) == kmin;
             const uint32_t vote = __ballot_sync(0xffffffffu, eq);
             const uint32_t m = __popc(vote);
             if (left <= m) {
@@ -394,16 +484,39 @@ sample_kernel(const SampleParams p) {
     }
   }
 
-  // ---- sums of the kept weights in index order
-  auto kept = [&](int i) -> unsigned long long {
-    const uint32_t k = sp_key(sx[i]);
-    return k > cut_key || (k == cut_key && lo + i <= cut_idx) ? weight(sx[i]) : 0ull;
+  // ---- sums of the kept weights in index order.  Where a cut leaves few, a warp lists them first; else lanes own neighbouring elements.
+  auto keep = [&](int i) {
+    const uint32_t k = sp_key(at(i));
+    return k > cut_key || (k == cut_key && lo + i <= cut_idx);
   };
-  __syncthreads();
+  __syncthreads();                                  // the candidates make room for the lists
+  uint16_t* list = s.w.list[warp];
+  int listed = -1;                                  // kept elements; -1: not listed
+  if (cut_key) {
+    listed = 0;
+#pragma unroll 2
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+      const bool k = i0 + lane < w1 && keep(i0 + lane);
+      const uint32_t vote = __ballot_sync(0xffffffffu, k);
+      const int to = listed + __popc(vote & ((1u << lane) - 1));
+      if (k && to < SP_LIST) list[to] = static_cast<uint16_t>(i0 + lane);
+      listed += __popc(vote);
+    }
+    if (listed > SP_LIST) listed = -1;
+    __syncwarp();
+  }
+  const int l0 = min(w1, w0 + lane * each), l1 = min(w1, l0 + each);
   unsigned long long mine = 0;
-  for (int i = w0 + lane; i < w1; i += 32) mine += kept(i);
-  mine = warp_sum64(mine);
-  if (lane == 0) s.red[warp] = mine;
+  if (listed >= 0) {
+    for (int i = lane; i < listed; i += 32) mine += weight(at(list[i]));
+  } else {
+#pragma unroll 1
+    for (int i = l0; i < l1; ++i) {
+      if (keep(i)) mine += weight(at(i));
+    }
+  }
+  const unsigned long long upto = warp_scan64(mine);            // with this lane
+  if (lane == 31) s.red[warp] = upto;
   __syncthreads();
   if (tid < C) {
     unsigned long long m = 0;
@@ -418,12 +531,23 @@ sample_kernel(const SampleParams p) {
   }
   for (int q = 0; q < warp; ++q) front += s.red[q];
   const unsigned long long target = min(static_cast<unsigned long long>(fmax(0.0, static_cast<double>(u) * static_cast<double>(sum))), sum - 1);
-  if (front > target || target >= front + mine) return;
-  for (int i0 = w0; i0 < w1; i0 += 32) {            // one warp of the row: walk its part
-    const unsigned long long run = front + warp_scan64(i0 + lane < w1 ? kept(i0 + lane) : 0ull);
-    const uint32_t vote = __ballot_sync(0xffffffffu, run > target);
-    if (vote) {
-      if (lane == __ffs(vote) - 1) p.out[row] = lo + i0 + lane;
+  const uint32_t vote = __ballot_sync(0xffffffffu, front + upto > target);
+  if (front > target || !vote) return;
+  // one warp of the row: 32 elements of its list, or of the lane that the number falls into, at a time
+  int from = 0, to = listed;
+  if (listed < 0) {
+    const int owner = __ffs(vote) - 1;
+    front += __shfl_sync(0xffffffffu, upto - mine, owner);
+    from = __shfl_sync(0xffffffffu, l0, owner);
+    to = __shfl_sync(0xffffffffu, l1, owner);
+  }
+  for (int i0 = from; i0 < to; i0 += 32) {
+    const int i = min(i0 + lane, to - 1), e = listed >= 0 ? list[i] : i;
+    const unsigned long long w = weight(at(e));
+    const unsigned long long run = front + warp_scan64(i0 + lane < to && (listed >= 0 || keep(e)) ? w : 0ull);
+    const uint32_t v = __ballot_sync(0xffffffffu, run > target);
+    if (v) {
+      if (lane == __ffs(v) - 1) p.out[row] = lo + e;
       return;
     }
     front = __shfl_sync(0xffffffffu, run, 31);
@@ -439,16 +563,20 @@ B200_API int b200_sample(const SampleParams* a, int B, int is_bf16, void* stream
   SampleParams p = *a;
   if (B <= 0 || p.V <= 0 || p.ld < p.V || !p.logits || !p.uniform || !p.out) return -1;
   int C = 1;
-  while (C < SP_MAX_CTAS && ((p.V + C - 1) / C > 8192 || (static_cast<long long>(B) * C < 296 && (p.V + C - 1) / C > 1024))) C *= 2;
+  // as many CTAs per row as the machine holds at a time (two per SM) and slices of more than 1024 elements allow; at most 40960 to a slice
+  while (C < 8 && ((p.V + C - 1) / C > 40960 || (static_cast<long long>(B) * 2 * C <= 296 && (p.V + C - 1) / C > 1024))) C *= 2;
+  if (C == 8 && B <= 4 && (p.V + C - 1) / C > 2048) C = 16;        // beyond the portable size, for few rows
   p.per = ((p.V + C - 1) / C + SP_THREADS - 1) / SP_THREADS * SP_THREADS;
-  const int smem = p.per * 4;
-  if (smem > 160 * 1024 || static_cast<long long>(B) * C > (1ll << 31) - 1) return -2;
+  const int smem = (p.per + p.per / 32) * 4;
+  if (smem > 180 * 1024 || static_cast<long long>(B) * C > (1ll << 31) - 1) return -2;
   auto kern = is_bf16 ? sample_kernel<__nv_bfloat16> : sample_kernel<float>;
   int dev = 0;
   static int configured[64][2] = {};
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   if (configured[dev][is_bf16 != 0] < smem) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -4;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return -4;
     configured[dev][is_bf16 != 0] = smem;
   }
   cudaLaunchConfig_t cfg = {};
