@@ -7,7 +7,8 @@ Design for B200:
 * the KV cache is a static ``[slots, B, Lmax, H_kv, D]`` tensor pair with one slot per (prelude block | recurrence step
   x core block | coda block) -- the per-recurrence-step cache of the reference -- optionally folded onto fewer slots
   (``compress-s{N}``); q/k bias + RoPE + cache append is one kernel, attention over the cache a split-K
-  flash-decoding kernel with per-sequence lengths;
+  flash-decoding kernel with per-sequence lengths; ``kv_dtype="fp8"`` keeps the same slots as 8-bit codes with one exponent per
+  head and block of tokens (``ops/kv8.py``): half the memory and half the bytes that a token's attention reads;
 * a whole token (prelude, r recurrences, coda, head, argmax, position bump) is ONE CUDA graph replay for fixed depth;
   with the KL exit each recurrence is a graph, the criterion (log-softmax, KL against the previous step, threshold,
   first-exit bookkeeping) runs in one kernel on the device, and the host looks at a single live-sequence counter
@@ -23,7 +24,10 @@ import ctypes as C
 
 import torch
 
+from ..models.sampling import SamplingOptions
 from ..ops import cuda as K
+from ..ops import kv8
+from ..ops.sampling import sample_tokens
 from .base import BF16, PDL, SKINNY_ROWS, GraphRunner, skinny_linear
 
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
@@ -74,10 +78,43 @@ class StaticRecurrentKVCache:
         return 2 * self.k.numel() * 2 / 2**20
 
 
+class StaticRecurrentKV8Cache(StaticRecurrentKVCache):
+    """The same slots in 8 bits: codes ``[slots, B, H_kv, capacity, D]`` and exponents ``[slots, B, H_kv, capacity / block]``; ``layers[s]``
+    is the ``KV8Cache`` of slot s.  The first chunk of a prompt is attended to as it is, in bf16; later ones read the decoded cache."""
+
+    def __init__(self, n_slots: int, batch: int, max_len: int, n_kv: int, head_dim: int, device, prelude: int, core: int,
+                 coda: int, compress: int = 0, block: int = 32):
+        self.P, self.R, self.Cn, self.compress = prelude, core, coda, compress
+        self.n_slots, self.max_len = n_slots, max_len
+        blocks = (max_len + block - 1) // block
+        self.k, self.v = (torch.zeros(n_slots, batch, n_kv, blocks * block, head_dim, dtype=torch.uint8, device=device).view(kv8.E4M3)
+                          for _ in range(2))
+        self.k_exp, self.v_exp = (torch.zeros(n_slots, batch, n_kv, blocks, dtype=torch.int8, device=device) for _ in range(2))
+        self.layers = [kv8.KV8Cache(self.k[s], self.v[s], self.k_exp[s], self.v_exp[s]) for s in range(n_slots)]
+        self._seen_tokens = 0
+
+    def update(self, k, v, step_idx, lookup_strategy=None):
+        step_idx = int(step_idx)
+        layer, n = self.layers[self.slot(step_idx)], k.shape[1]
+        if step_idx == 0:
+            self._seen_tokens += n
+        end = self._seen_tokens
+        kv8.append(layer, k, v, torch.full((k.shape[0],), end - n, dtype=torch.int32, device=k.device))
+        if end == n:
+            return k, v
+        k, v = layer.decoded()
+        return k[:, :end], v[:, :end]
+
+    def get_memory_usage(self) -> float:
+        return sum(t.numel() for t in (self.k, self.v, self.k_exp, self.v_exp)) / 2**20
+
+
 class DecodeEngine(GraphRunner):
     def __init__(self, model, max_batch: int, max_len: int, num_steps: int | None = None,
                  cache_lookup_strategy: str = "full", use_graphs: bool = True, attn_splits: int = 0,
-                 max_steps: int | None = None):
+                 max_steps: int | None = None, kv_dtype: str = "bf16"):
+        if kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"kv_dtype is 'bf16' or 'fp8': got {kv_dtype!r}")
         cfg = model.config
         self.model, self.cfg = model, cfg
         self.dev = next(model.parameters()).device
@@ -93,14 +130,18 @@ class DecodeEngine(GraphRunner):
             compress = int(cache_lookup_strategy.split("compress-s")[1].split("-")[0])
         self.max_steps = max(self.r, max_steps or self.r)  # cache slots exist for this many recurrences
         rec_slots = compress if compress else self.R * self.max_steps
-        self.cache = StaticRecurrentKVCache(self.P + rec_slots + self.Cn, max_batch, max_len, self.Hkv, self.D,
-                                            self.dev, self.P, self.R, self.Cn, compress)
+        self.kv8 = kv_dtype == "fp8"
+        cache_class = StaticRecurrentKV8Cache if self.kv8 else StaticRecurrentKVCache
+        self.cache = cache_class(self.P + rec_slots + self.Cn, max_batch, max_len, self.Hkv, self.D, self.dev, self.P, self.R, self.Cn, compress)
         self.use_graphs = use_graphs
         # flash-decoding splits of the key range: enough CTAs (128 threads each) to fill every SM's thread slots at small
         # batch -- the per-key walk is latency-bound, so more, shorter walks win (B=1: 16 splits, B=8: 5, B>=32: 1)
         self.splits = attn_splits or max(1, min(16, (16 * 148) // max(1, max_batch * self.H)))
         cos, sin = model._rope(max_len)
         self.cos, self.sin = cos.float().contiguous(), sin.float().contiguous()
+        if self.kv8:      # tables reach to the end of the last block, whose last positions are never met
+            more = self.cache.layers[0].capacity - max_len
+            self.cos, self.sin = (torch.cat([t, t[-1:].expand(more, -1)]).contiguous() for t in (self.cos, self.sin))
         d = self.dev
         self.pos = torch.zeros(max_batch, dtype=torch.int32, device=d)
         self.lens = torch.zeros(max_batch, dtype=torch.int32, device=d)
@@ -111,6 +152,7 @@ class DecodeEngine(GraphRunner):
         self.state_out = torch.zeros_like(self.state)
         self.init_buf = torch.zeros_like(self.state)                            # fresh random state per token
         self.tok_out = torch.zeros(max_batch, dtype=torch.int64, device=d)
+        self.uniform = torch.zeros(max_batch, dtype=torch.float32, device=d)   # numbers that the next token is drawn from
         self.next_state = torch.zeros_like(self.state)
         self._seed = 1
         self.logits = torch.zeros(max_batch, self.V, dtype=torch.float32, device=d)
@@ -167,6 +209,13 @@ class DecodeEngine(GraphRunner):
     def _attention(self, attn, h, slot: int):
         B = h.shape[0]
         qkv = self._linear(h, attn.Wqkv.weight, keep_f32=True)   # bf16, or the fp32 stream-K accumulator
+        if self.kv8:
+            layer = self.cache.layers[slot]
+            bias = self._bias(attn)
+            q = kv8.rope_append(layer, qkv, self.cos, self.sin, self.pos, self.H, None if bias is None else bias.view(-1)[:(self.H + self.Hkv) * self.D],
+                                clear=qkv.dtype == torch.float32)
+            o = kv8.attention(q[:, None], layer, self.lens, max_len=self.Lmax)
+            return self._linear(o.view(B, self.H * self.D), attn.proj.weight, keep_f32=True)
         q = torch.empty(B, self.H * self.D, dtype=BF16, device=h.device)
         kc, vc = self.cache.k[slot], self.cache.v[slot]
         bias = self._bias(attn)
@@ -235,8 +284,22 @@ class DecodeEngine(GraphRunner):
             self.init_buf.copy_(K.trunc_normal(self.init_buf.shape, std, self._seed, BF16, self.dev))
 
     # -- public API ---------------------------------------------------------------------------------------
+    @staticmethod
+    def _settings(sampling: SamplingOptions | None) -> dict | None:
+        """Arguments of ``sample_tokens``; None: greedy."""
+        if sampling is None or sampling.greedy:
+            return None
+        if sampling.repetition_penalty not in (None, 1.0):
+            raise ValueError("the recurrent decode engine has no repetition penalty")
+        return dict(temperature=float(sampling.temperature or 1.0), top_k=int(sampling.top_k or 0), top_p=float(sampling.top_p or 1.0),
+                    min_p=float(sampling.min_p or 0.0))
+
+    def _pick(self, logits, settings: dict | None):
+        return logits.argmax(-1) if settings is None else sample_tokens(logits, self.uniform[:logits.shape[0]], **settings)
+
     @torch.no_grad()
-    def prefill(self, input_ids: torch.Tensor, num_steps: int | None = None, init_scale: float = 1.0):
+    def prefill(self, input_ids: torch.Tensor, num_steps: int | None = None, init_scale: float = 1.0,
+                sampling: SamplingOptions | None = None):
         """Process the prompt with the ordinary (large-M) kernels, filling every cache slot; returns the first
         generated token and the last-position latent."""
         B, P = input_ids.shape
@@ -244,13 +307,13 @@ class DecodeEngine(GraphRunner):
         self.cache._seen_tokens = 0
         out = self.model(input_ids, num_steps=num_steps or self.r, use_cache=True, past_key_values=self.cache,
                          cache_position=torch.arange(P, device=self.dev), init_scale=init_scale)
-        self.tok.copy_(out.logits[:, -1, :].argmax(-1))
+        self.tok.copy_(self._pick(out.logits[:, -1, :], self._settings(sampling)))
         self.state.copy_(out.latent_states[:, -1, :])
         self.pos.fill_(P)
         self.lens.fill_(P + 1)
         return self.tok.clone()
 
-    def _token_fixed(self, r: int, continuous: bool):
+    def _token_fixed(self, r: int, continuous: bool, settings: dict | None = None):
         """Graph body: token ``tok`` at position ``pos`` -> ``tok_out`` / ``state_out`` (inputs are not modified)."""
         e = self._embed()
         s = self.state if continuous else self.init_buf
@@ -258,26 +321,36 @@ class DecodeEngine(GraphRunner):
             s = self._recurrence(s, e, step)
         logits = self._head(s)
         self.state_out.copy_(s)
-        self.tok_out.copy_(logits.argmax(-1))
+        self.tok_out.copy_(self._pick(logits, settings))
         return self.tok_out
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, num_steps: int | None = None,
                  criterion: str | None = None, exit_threshold: float = 5e-4, max_steps: int | None = None,
-                 continuous_compute: bool = False, init_scale: float = 1.0, check_every: int = 4, min_steps: int = 0):
-        """Greedy decoding.  ``criterion=None``: fixed ``num_steps`` recurrences per token.  ``criterion="kl"``: KL
-        exit with ``exit_threshold`` and at most ``max_steps`` recurrences.  Returns (tokens [B, P+new], stats)."""
+                 continuous_compute: bool = False, init_scale: float = 1.0, check_every: int = 4, min_steps: int = 0,
+                 sampling: SamplingOptions | None = None, generator: torch.Generator | None = None):
+        """Decoding, greedy unless ``sampling`` says otherwise.  ``criterion=None``: fixed ``num_steps`` recurrences per token.
+        ``criterion="kl"``: KL exit with ``exit_threshold`` and at most ``max_steps`` recurrences (greedy only).  Sampled tokens are
+        drawn from uniform numbers of ``generator`` (a generator of the engine's device).  Returns (tokens [B, P+new], stats)."""
         r = num_steps or self.r
         B, P = input_ids.shape
         assert P + max_new_tokens <= self.Lmax
-        first = self.prefill(input_ids, r, init_scale)
+        settings = self._settings(sampling)
+        if settings is not None and criterion is not None:
+            raise ValueError("sampling goes with a fixed number of recurrences")
+        if settings is not None:
+            self.uniform.uniform_(generator=generator)
+        first = self.prefill(input_ids, r, init_scale, sampling)
         out = [first]
         steps_log = []
         if criterion is None:
             for _ in range(max_new_tokens - 1):
                 if not continuous_compute:
                     self._fresh_state(init_scale)
-                self._run(("fixed", r, continuous_compute), lambda: self._token_fixed(r, continuous_compute))
+                if settings is not None:
+                    self.uniform.uniform_(generator=generator)
+                key = ("fixed", r, continuous_compute) + (() if settings is None else tuple(settings.values()))
+                self._run(key, lambda: self._token_fixed(r, continuous_compute, settings))
                 self.tok.copy_(self.tok_out)
                 self.state.copy_(self.state_out)
                 self.pos.add_(1)

@@ -3,7 +3,8 @@
 Role of the reference's vLLM plugin (vllm/raven_vllm.py:297-411 fixed-recurrence model, :471-542 weight loading,
 vllm/README.md:19-24 data-parallel replicas).  That plugin is a library path (vLLM's scheduler, attention and paged
 cache) with a fixed recurrence; here the product is the native engine (`engine/decode.py`): per-step static KV cache,
-CUDA-graphed recurrence, latent reuse and device-side KL exit, so the adaptive-depth options are served too.
+CUDA-graphed recurrence, latent reuse and device-side KL exit, so the adaptive-depth options are served too; tokens are greedy or
+sampled on the device, and the cache may be held in 8 bits.
 
 Pieces:
   * ``EngineBackend``  — a ``DecodeEngine`` on one GPU (bf16).
@@ -25,6 +26,8 @@ from dataclasses import dataclass, field
 from typing import Optional
 
 import torch
+
+from ..models.sampling import SamplingOptions
 
 
 @dataclass
@@ -100,23 +103,23 @@ class EngineBackend:
     ragged = False
 
     def __init__(self, model, max_batch: int = 8, max_len: int = 4096, max_steps: int | None = None,
-                 cache_lookup_strategy: str = "full"):
+                 cache_lookup_strategy: str = "full", kv_dtype: str = "bf16"):
         from .decode import DecodeEngine
 
         self.engine = DecodeEngine(model, max_batch=max_batch, max_len=max_len, max_steps=max_steps,
-                                   cache_lookup_strategy=cache_lookup_strategy)
+                                   cache_lookup_strategy=cache_lookup_strategy, kv_dtype=kv_dtype)
         self.max_batch, self.device = max_batch, self.engine.dev
         self.name = "decode-engine"
 
     @torch.no_grad()
     def generate(self, prompts: list, opt: DecodeOptions):
-        if opt.sampling():
-            raise ValueError("the recurrent decode engine decodes greedily")
+        sampling = SamplingOptions(**opt.sampling())
         rows = prompts + [prompts[0]] * (self.max_batch - len(prompts))
         ids = torch.tensor(rows, dtype=torch.long, device=self.device)
         tokens, stats = self.engine.generate(ids, opt.max_tokens, num_steps=opt.num_steps, criterion=opt.criterion,
                                              exit_threshold=opt.exit_threshold, max_steps=opt.max_steps,
-                                             continuous_compute=opt.continuous_compute, init_scale=opt.init_scale)
+                                             continuous_compute=opt.continuous_compute, init_scale=opt.init_scale,
+                                             sampling=sampling)
         if stats.get("device_status"):
             raise RuntimeError(f"decode kernels reported device status {stats['device_status']}")
         P = len(prompts[0])
@@ -153,14 +156,17 @@ class LayeredBackend:
 
 
 def make_backend(model, max_batch: int = 8, max_len: int = 4096, max_steps: int | None = None,
-                 cache_lookup_strategy: str = "full", stop_ids=None):
+                 cache_lookup_strategy: str = "full", stop_ids=None, kv_dtype: str = "bf16"):
     """The backend that serves ``model`` on the device it lies on."""
     from ..models.layered import LayeredForCausalLM
 
-    if isinstance(model, LayeredForCausalLM):
+    recurrent = not isinstance(model, LayeredForCausalLM)
+    if kv_dtype != "bf16" and not (recurrent and next(model.parameters()).is_cuda):
+        raise ValueError("an 8-bit key / value cache belongs to the recurrent decode engine on a GPU")
+    if not recurrent:
         return LayeredBackend(model, max_batch, max_len, stop_ids or ())
     if next(model.parameters()).is_cuda:
-        return EngineBackend(model, max_batch, max_len, max_steps, cache_lookup_strategy)
+        return EngineBackend(model, max_batch, max_len, max_steps, cache_lookup_strategy, kv_dtype)
     return ModelBackend(model, max_batch)
 
 

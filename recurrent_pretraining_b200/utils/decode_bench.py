@@ -2,7 +2,7 @@
 greedy, r = 32 with the per-recurrence-step KV cache; optional KL exit (5e-4, max r 64) with latent reuse.
 
 ``python -m recurrent_pretraining_b200.utils.decode_bench [--batches 1,8,32,64] [--new 256] [--prompt 512] [--kl]
-[--eager] [--reference]``.  Device-timed with CUDA events around the generation loop (prefill excluded and reported
+[--kv-dtype fp8] [--eager] [--reference]``.  Device-timed with CUDA events around the generation loop (prefill excluded and reported
 separately); weights are random-init.  ``--eager`` times this repository's HF-style token loop, ``--reference`` the
 unmodified reference HF model in a hand-written cached loop (its ``generate`` no longer runs under transformers 5).
 """
@@ -49,6 +49,7 @@ def main():
     ap.add_argument("--eager", action="store_true")
     ap.add_argument("--reference", action="store_true")
     ap.add_argument("--cache", default="full")
+    ap.add_argument("--kv-dtype", choices=["bf16", "fp8"], default="bf16")
     ap.add_argument("--profile", action="store_true", help="print per-kernel time shares of a few decode tokens")
     args = ap.parse_args()
     from ..engine.decode import DecodeEngine
@@ -58,10 +59,10 @@ def main():
     for B in [int(b) for b in args.batches.split(",")]:
         ids = torch.randint(0, V - 100, (B, args.prompt), device="cuda")
         rec = {"model": args.model, "batch": B, "prompt": args.prompt, "new_tokens": args.new, "r": args.steps,
-               "cache": args.cache}
+               "cache": args.cache, "kv_dtype": args.kv_dtype}
         max_steps = 64 if args.kl else args.steps
         eng = DecodeEngine(model, B, args.prompt + args.new + 1, num_steps=args.steps, cache_lookup_strategy=args.cache,
-                           max_steps=max_steps)
+                           max_steps=max_steps, kv_dtype=args.kv_dtype)
         rec["kv_cache_GiB"] = round(eng.cache.get_memory_usage() / 1024, 2)
         kw = dict(criterion="kl", exit_threshold=5e-4, max_steps=64, continuous_compute=True) if args.kl else {}
         eng.generate(ids, 4, **kw)  # warm-up: graph capture

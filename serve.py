@@ -46,7 +46,7 @@ def run_replica(args):
 
         tokenizer = Tokenizer(args.tokenizer)
     stops = [int(x) for x in args.stop_ids.split(",") if x] if args.stop_ids is not None else None
-    backend = make_backend(model, args.max_batch, args.max_len, args.max_steps, args.cache_lookup_strategy, stops)
+    backend = make_backend(model, args.max_batch, args.max_len, args.max_steps, args.cache_lookup_strategy, stops, args.kv_cache)
     if stops is None:
         stops = () if backend.ragged else RAVEN_STOP_IDS
     sched = BatchScheduler(backend, window_ms=args.batch_window_ms, stop_ids=stops)
@@ -111,6 +111,7 @@ def main(argv=None):
     ap.add_argument("--max-len", type=int, default=4096)
     ap.add_argument("--max-steps", type=int, default=None, help="recurrence cap the KV cache is sized for")
     ap.add_argument("--cache-lookup-strategy", default="full")
+    ap.add_argument("--kv-cache", choices=["bf16", "fp8"], default="bf16", help="storage of the recurrent engine's keys and values")
     ap.add_argument("--batch-window-ms", type=float, default=3.0)
     ap.add_argument("--cpu", action="store_true", help="serve through model.generate on CPU (debug)")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default=None, help="default: bfloat16 on a GPU, float32 on CPU")

@@ -1,0 +1,125 @@
+"""The recurrent decode engine over the 8-bit cache and with sampled tokens, and the serving layer's options for both."""
+import pytest
+import torch
+
+from recurrent_pretraining_b200.config import ModelConfig
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def model():
+    from recurrent_pretraining_b200.models.hf import RavenForCausalLM
+
+    torch.manual_seed(0)
+    cfg = ModelConfig.from_name("smoke-raven-96", mean_recurrence=4)
+    return RavenForCausalLM.from_training_model(cfg.construct_model()).to(torch.bfloat16).cuda().eval()
+
+
+@gpu
+@pytest.mark.parametrize("use_graphs,B,P,strategy", [(False, 2, 24, "full"), (True, 3, 41, "full"), (True, 2, 33, "full-compress-s4")])
+def test_engine_over_the_8bit_cache(model, use_graphs, B, P, strategy):
+    """The engine's tokens are (nearly) the largest logits of a cache whose values were rounded to e4m3: the eager model on the engine's
+    own tokens differs by that rounding, whose effect on these logits is far below their spread."""
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+
+    torch.manual_seed(1)
+    new = 9
+    ids = torch.randint(0, 4000, (B, P), device="cuda")
+    eng = DecodeEngine(model, max_batch=B, max_len=61, num_steps=4, use_graphs=use_graphs, cache_lookup_strategy=strategy, kv_dtype="fp8")
+    toks, stats = eng.generate(ids, new, init_scale=0.0)
+    assert stats["device_status"] == 0 and toks.shape == (B, P + new)
+    if "compress" not in strategy:
+        pred = model(toks[:, :-1], num_steps=4, init_scale=0.0).logits[:, P - 1:, :].float()
+        chosen = torch.gather(pred, -1, toks[:, P:].unsqueeze(-1)).squeeze(-1)
+        assert bool((chosen >= pred.max(-1).values - 0.15 - 0.25 * pred.std(-1)).all())
+    again, _ = eng.generate(ids, new, init_scale=0.0)      # reused rows need no clearing
+    assert torch.equal(again, toks)
+    half = DecodeEngine(model, max_batch=B, max_len=61, num_steps=4, cache_lookup_strategy=strategy)
+    assert eng.cache.get_memory_usage() < 0.56 * half.cache.get_memory_usage()
+
+
+@gpu
+def test_graphs_over_the_8bit_cache_change_nothing(model):
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+
+    ids = torch.randint(0, 4000, (3, 30), device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    outs = [DecodeEngine(model, 3, 64, num_steps=4, use_graphs=g, kv_dtype="fp8").generate(ids, 12, init_scale=0.0)[0] for g in (False, True)]
+    assert torch.equal(*outs)
+
+
+@gpu
+def test_kl_exit_and_programmatic_launch_over_the_8bit_cache(model, monkeypatch):
+    from recurrent_pretraining_b200.engine import decode as D
+
+    torch.manual_seed(2)
+    ids = torch.randint(0, 4000, (2, 16), device="cuda")
+    eng = D.DecodeEngine(model, max_batch=2, max_len=48, num_steps=4, max_steps=8, kv_dtype="fp8")
+    toks, reuse = eng.generate(ids, 4, criterion="kl", exit_threshold=5e-4, max_steps=8, continuous_compute=True)
+    assert toks.shape == (2, 20) and reuse["device_status"] == 0
+    plain, _ = eng.generate(ids, 8, init_scale=0.0)
+    monkeypatch.setattr(D, "PDL", True)
+    toks, stats = D.DecodeEngine(model, max_batch=2, max_len=48, num_steps=4, max_steps=8, kv_dtype="fp8").generate(ids, 8, init_scale=0.0)
+    assert stats["device_status"] == 0 and torch.equal(toks, plain)
+
+
+@gpu
+def test_a_prompt_in_two_chunks_reads_the_decoded_cache(model):
+    from recurrent_pretraining_b200.engine.decode import StaticRecurrentKV8Cache
+
+    cache = StaticRecurrentKV8Cache(3, 2, 50, 5, 96, "cuda", 2, 4, 2)
+    k = torch.randn(2, 40, 5, 96, device="cuda").to(torch.bfloat16)
+    a, _ = cache.update(k[:, :25], k[:, :25], 0)
+    assert a.data_ptr() == k.data_ptr()
+    b, c = cache.update(k[:, 25:], -k[:, 25:], 0)
+    assert b.shape == (2, 40, 5, 96)
+    assert ((b.float() - k.float()).abs() <= 2.0 ** -4 * k.float().abs() + 2.0 ** -9).all()     # one rounding to e4m3, or two where a block grew
+    assert ((c[:, 25:].float() + k[:, 25:].float()).abs() <= 2.0 ** -4 * k[:, 25:].float().abs() + 2.0 ** -9).all()
+
+
+@gpu
+@pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
+def test_sampled_tokens(model, kv_dtype):
+    """Sampling is what ``sample_tokens`` draws from the engine's own logits; a generator repeats it, and the narrowest filters are greedy."""
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+    from recurrent_pretraining_b200.models.sampling import SamplingOptions
+
+    ids = torch.randint(0, 4000, (2, 20), device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    eng = DecodeEngine(model, max_batch=2, max_len=64, num_steps=4, kv_dtype=kv_dtype)
+    run = lambda seed, **o: eng.generate(ids, 10, init_scale=0.0, sampling=SamplingOptions(do_sample=True, **o),  # noqa: E731
+                                         generator=torch.Generator("cuda").manual_seed(seed))[0]
+    greedy = eng.generate(ids, 10, init_scale=0.0)[0]
+    assert torch.equal(run(1, top_k=1), greedy) and torch.equal(run(2, top_p=1e-9), greedy) and torch.equal(run(3, min_p=1.0), greedy)
+    a = run(7, temperature=1.5, top_k=200, top_p=0.95)
+    assert torch.equal(a, run(7, temperature=1.5, top_k=200, top_p=0.95)) and not torch.equal(a, run(8, temperature=1.5, top_k=200, top_p=0.95))
+    assert torch.equal(eng.generate(ids, 10, init_scale=0.0, sampling=SamplingOptions(temperature=3.0))[0], greedy)      # do_sample is off
+    with pytest.raises(ValueError):
+        eng.generate(ids, 4, criterion="kl", sampling=SamplingOptions(do_sample=True))
+    with pytest.raises(ValueError):
+        eng.generate(ids, 4, sampling=SamplingOptions(do_sample=True, repetition_penalty=1.2))
+
+
+@gpu
+def test_served_with_sampling_over_the_8bit_cache(model):
+    from recurrent_pretraining_b200.engine import server as S
+
+    sched = S.BatchScheduler(S.make_backend(model, max_batch=2, max_len=64, kv_dtype="fp8"), window_ms=20.0, stop_ids=())
+    try:
+        body = {"prompt": [5, 17, 3], "max_tokens": 6, "num_steps": 4, "init_scale": 0.0}
+        greedy = S.handle_completion(sched, body)["choices"][0]["token_ids"]
+        assert S.handle_completion(sched, {**body, "do_sample": True, "top_k": 1})["choices"][0]["token_ids"] == greedy
+        assert len(S.handle_completion(sched, {**body, "do_sample": True, "temperature": 0.8, "top_p": 0.9})["choices"][0]["token_ids"]) == 6
+        with pytest.raises(RuntimeError):
+            S.handle_completion(sched, {**body, "do_sample": True, "criterion": "kl"})
+    finally:
+        sched.close()
+
+
+def test_an_8bit_cache_is_refused_where_there_is_none():
+    from recurrent_pretraining_b200.engine import server as S
+
+    class Tiny(torch.nn.Linear):
+        pass
+
+    with pytest.raises(ValueError):
+        S.make_backend(Tiny(2, 2), kv_dtype="fp8")
