@@ -12,7 +12,9 @@
 // and divided further by the bits of their keys until few are left, which are ranked against each other.  Should they be too many to be
 // collected (equal logits), the whole slices are divided again, down to a single value whose ties are counted in index order.
 //
-// A row is bound by the latency of its stages, which the machine runs side by side for a batch: TODO_FIG
+// A row is bound by the latency of its stages: 17.5 us for 65536 fp32 logits with top-k 50 and top-p 0.9 (16 CTAs; read 1.6, maximum 0.8,
+// histogram 3, its exchange 3, candidates 2, ranking 2.5, kept list and its sums 2, the token 2), where 8 CTAs take 24 and the bytes 0.04.  A batch
+// of 64 such rows (4 CTAs each, two per SM) takes 41.5 us: it is bound by the instructions of the pass that forms the weights and the histogram.
 #include <cooperative_groups.h>
 
 #include <utility>
@@ -23,7 +25,9 @@ namespace b200 {
 namespace cg = cooperative_groups;
 
 constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_BINS = 512, SP_CAND = 1024, SP_FEW = 128, SP_MAX_CTAS = 16, SP_TAB = 256, SP_LIST = 512;
+constexpr int SP_SEG = SP_THREADS / SP_FEW;         // threads that rank a candidate
 constexpr float SP_BINS_PER_OCTAVE = 32.f;
+constexpr int SP_MAX_SMEM = 180 * 1024;             // for the slice
 constexpr int SP_ONE = 44;                          // a weight of 1 is 2^44; 2^18 of them fit the sums
 static_assert(SP_BINS == SP_THREADS, "a bin per thread");
 
@@ -40,20 +44,22 @@ struct SampleParams {
 };
 
 struct SampleHist {
-  uint32_t cnt[SP_BINS], lo[SP_BINS], hi[SP_BINS];  // sums of weights as two words
+  uint32_t cnt[SP_BINS];
+  struct alignas(8) { uint32_t lo, hi; } mass[SP_BINS];     // sums of weights as two words
 };
 struct SampleShared {
-  union {
-    SampleHist hist;                                // this slice
-    struct { uint32_t key[SP_CAND], idx[SP_CAND]; } sel;        // the last few candidates, when all CTAs have read the histogram
-  } h;
+  SampleHist hist;                                  // this slice
   uint32_t key[SP_CAND], idx[SP_CAND];              // candidates of this slice
   union {
     struct {
-      uint32_t key[SP_CAND], idx[SP_CAND];          // of the row
+      uint32_t key[SP_CAND], idx[SP_CAND];          // of the row, SP_CAND / CTAs places for each slice; key 0: none
       union {
         SampleHist sub;
-        unsigned long long sorted[SP_CAND];
+        struct {                                    // the last few: keys, indices, weights, and what each quarter of them puts in front
+          uint32_t key[SP_FEW], idx[SP_FEW];
+          unsigned long long w[SP_FEW], sum[SP_SEG][SP_FEW];
+          uint32_t rank[SP_SEG][SP_FEW];
+        } few;
       } u;
     } all;
     uint16_t list[SP_WARPS][SP_LIST];               // kept elements of a warp's part, in order
@@ -62,8 +68,9 @@ struct SampleShared {
   unsigned long long red[SP_WARPS], red2[SP_WARPS];
   unsigned long long xch[2][SP_MAX_CTAS];           // what the CTAs of the cluster tell each other
   uint32_t xa[2][SP_MAX_CTAS], xb[2][SP_MAX_CTAS];
-  uint32_t ncand, nsel, order[SP_FEW];
-  int found, found2;
+  uint32_t ncand, nsel;
+  int found, found2, cut_idx;
+  uint32_t cut_k, cut_p;
   unsigned long long before[2];
 };
 
@@ -89,18 +96,18 @@ __device__ __forceinline__ unsigned long long warp_scan64(unsigned long long v) 
 
 // w to a bin of a histogram; the carry of the lower word goes to the upper one, so the sum is exact whatever the order.
 __device__ __forceinline__ void sp_add(SampleHist& h, int bin, unsigned long long w) {
-  const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&h.lo[bin], l);
+  const uint32_t l = static_cast<uint32_t>(w), old = atomicAdd(&h.mass[bin].lo, l);
   const uint32_t up = static_cast<uint32_t>(w >> 32) + (old + l < old ? 1u : 0u);
-  if (up) atomicAdd(&h.hi[bin], up);
+  if (up) atomicAdd(&h.mass[bin].hi, up);
 }
+__device__ __forceinline__ unsigned long long sp_mass(const SampleHist& h, int bin) { return *reinterpret_cast<const unsigned long long*>(&h.mass[bin]); }
 
 struct SampleScale {
   float mx, cf;
   double c, mxc;                                    // log2(e) / T; max times that
 };
-// 2^-y, y = (max - v) log2(e) / T = a + i / 256 + r, in units of 2^-44.  Not inlined: a row runs through every stage of the kernel once,
-// and with eight copies of this in it the fetching of instructions took a third of its time.
-__device__ __noinline__ unsigned long long sp_weight(float v, float mx, float cf, double c, double mxc, const double* tab) {
+// 2^-y, y = (max - v) log2(e) / T = a + i / 256 + r, in units of 2^-44.
+__device__ __forceinline__ unsigned long long sp_weight_inline(float v, float mx, float cf, double c, double mxc, const double* tab) {
   const double y = fma(-static_cast<double>(v), c, mxc);
   const double big = 6755399441055744.0 / SP_TAB;   // 1.5 * 2^52 / 256: adding it leaves round(256 y) in the low bits
   const double z = y + big;
@@ -108,9 +115,15 @@ __device__ __noinline__ unsigned long long sp_weight(float v, float mx, float cf
   const double r = y - (z - big);                   // |r| <= 2^-9; 2^-r = 1 - z + z^2 / 2 - z^3 / 6, z = r ln 2, to 2e-13
   const double e = fma(r, fma(r, fma(r, -0.055504108664821580, 0.24022650695910071), -0.69314718055994531), 1.0);
   const double f = fma(tab[q & (SP_TAB - 1)], e, 4503599627370496.0);           // 2^52: the low bits are the rounded integer
-  const unsigned long long w = (static_cast<unsigned long long>(__double_as_longlong(f)) & 0xFFFFFFFFFFFFFull) >> (q / SP_TAB & 63);
+  const unsigned long long w = (static_cast<unsigned long long>(__double_as_longlong(f)) & 0xFFFFFFFFFFFFFull) >> (q >> 8 & 63);
   return v == mx ? 1ull << SP_ONE : (mx - v) * cf < SP_ONE + 1.f ? w : 0ull;    // (infinities, too)
 }
+// Not inlined where speed does not ask for it: a row runs through every stage of the kernel once, and with eight copies of this in it the
+// fetching of instructions took a third of its time.
+__device__ __noinline__ unsigned long long sp_weight(float v, float mx, float cf, double c, double mxc, const double* tab) {
+  return sp_weight_inline(v, mx, cf, c, mxc, tab);
+}
+static_assert(SP_TAB == 256, "shifts by eight above");
 
 template <typename T>
 __global__ void __launch_bounds__(SP_THREADS, 2)
@@ -128,7 +141,11 @@ sample_kernel(const SampleParams p) {
 
   auto started = cluster.barrier_arrive();          // before the first access to another CTA's memory it has to be running
   if (tid < SP_TAB) s.tab[tid] = exp2(static_cast<double>(SP_ONE) - tid / static_cast<double>(SP_TAB));
-  s.h.hist.cnt[tid] = s.h.hist.lo[tid] = s.h.hist.hi[tid] = 0;
+  auto clear = [&]() {                              // before a histogram, and before candidates arrive
+    s.hist.cnt[tid] = s.hist.mass[tid].lo = s.hist.mass[tid].hi = 0;
+    for (int i = tid; i < SP_CAND; i += SP_THREADS) s.w.all.key[i] = 0;
+  };
+  clear();
   pdl_trigger();
   pdl_wait();
   const T* x = static_cast<const T*>(p.logits) + static_cast<long long>(row) * p.ld + lo;
@@ -250,38 +267,46 @@ sample_kernel(const SampleParams p) {
       // most tokens of a vocabulary are improbable and share the last bin: they are added up in registers
       uint32_t rest = 0;
       unsigned long long rest_w = 0;
-#pragma unroll 2
+#pragma unroll 4
       for (int i = w0 + lane; i < w1; i += 32) {
         const float v = at(i);
         const int bin = bin_of(v);
-        const unsigned long long w = by_p ? weight(v) : 0ull;
+        const unsigned long long w = by_p ? sp_weight_inline(v, sc.mx, sc.cf, sc.c, sc.mxc, s.tab) : 0ull;
         if (bin == SP_BINS - 1) {
           ++rest;
           rest_w += w;
         } else if (bin >= 0) {
-          if (by_k) atomicAdd(&s.h.hist.cnt[bin], 1u);
-          if (w) sp_add(s.h.hist, bin, w);
+          if (by_k) atomicAdd(&s.hist.cnt[bin], 1u);
+          if (w) sp_add(s.hist, bin, w);
         }
       }
       rest = __reduce_add_sync(0xffffffffu, rest);
       rest_w = warp_sum64(rest_w);
       if (lane == 0 && rest) {
-        atomicAdd(&s.h.hist.cnt[SP_BINS - 1], rest);
-        sp_add(s.h.hist, SP_BINS - 1, rest_w);
+        atomicAdd(&s.hist.cnt[SP_BINS - 1], rest);
+        sp_add(s.hist, SP_BINS - 1, rest_w);
       }
       if (tid == 0) s.ncand = 0;
       cluster.sync();
-      uint32_t cnt_b = 0;
-      unsigned long long mass_b = 0;
-#pragma unroll 4
-      for (int q = 0; q < C; ++q) {
-          const SampleHist& h = cluster.map_shared_rank(&s, q)->h.hist;
-          if (by_k) cnt_b += h.cnt[tid];
-          if (by_p) mass_b += (static_cast<unsigned long long>(h.hi[tid]) << 32) + h.lo[tid];
+      {                                             // the slices' sums of a share of the bins, handed to every CTA: 8 KB to move, not 64
+        const int q = tid & (C - 1), bin = rank * (SP_BINS / C) + tid / C;
+        const SampleHist& h = cluster.map_shared_rank(&s, q)->hist;
+        uint32_t cnt = h.cnt[bin];
+        unsigned long long mass = sp_mass(h, bin);
+        for (int o = C >> 1; o > 0; o >>= 1) {
+          cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+          mass += __shfl_xor_sync(0xffffffffu, mass, o);
         }
+        SampleHist& sum = cluster.map_shared_rank(&s, q)->w.all.u.sub;
+        sum.cnt[bin] = cnt;
+        *reinterpret_cast<unsigned long long*>(&sum.mass[bin]) = mass;
+      }
+      cluster.sync();
+      const uint32_t cnt_b = s.w.all.u.sub.cnt[tid];
+      const unsigned long long mass_b = sp_mass(s.w.all.u.sub, tid);
       const int hit = crossing(cnt_b, mass_b, first);
       if (hit == SP_BINS) break;                    // the rest passes no limit (the same in all CTAs)
-      // ---- the bin's candidates, as far as they fit
+      // ---- the bin's candidates: listed, then handed to every CTA
 #pragma unroll 2
       for (int i = w0 + lane; i < w1; i += 32) {
         const float v = at(i);
@@ -290,54 +315,43 @@ sample_kernel(const SampleParams p) {
           if (slot < SP_CAND) { s.key[slot] = sp_key(v); s.idx[slot] = lo + i; }
         }
       }
-      cluster.sync();
-      // where the slices' candidates end: lane q has that of slice q
-      uint32_t end = lane < C ? cluster.map_shared_rank(&s, lane)->ncand : 0u;
-#pragma unroll
-      for (int o = 1; o < SP_MAX_CTAS; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, end, o);
-        if (lane >= o) end += up;
+      __syncthreads();
+      const uint32_t room = SP_CAND / C, found = s.ncand;
+      for (uint32_t i = tid; i < C * min(found, room); i += SP_THREADS) {
+        SampleShared* r = cluster.map_shared_rank(&s, i & (C - 1));
+        const uint32_t j = i / C;
+        r->w.all.key[rank * room + j] = s.key[j];
+        r->w.all.idx[rank * room + j] = s.idx[j];
       }
-      const uint32_t cand = __shfl_sync(0xffffffffu, end, SP_MAX_CTAS - 1);
-      if (cand <= SP_CAND) {
-        // ---- all of them in every CTA
-        for (uint32_t i0 = 32 * warp; i0 < cand; i0 += SP_THREADS) {
-          const uint32_t i = i0 + lane;
-          uint32_t from = 0;
-          int q = 0;
-#pragma unroll 1
-          for (int j = 0; j < C - 1; ++j) {
-            const uint32_t e = __shfl_sync(0xffffffffu, end, j);
-            if (i >= e) { q = j + 1; from = e; }
-          }
-          if (i < cand) {
-            const SampleShared* r = cluster.map_shared_rank(&s, q);
-            s.w.all.key[i] = r->key[i - from];
-            s.w.all.idx[i] = r->idx[i - from];
-          }
-        }
-        __syncthreads();
+      if (tid < C) cluster.map_shared_rank(&s, tid)->xa[phase][rank] = found;
+      cluster.sync();
+      uint32_t left = 0, most = 0;
+      for (int q = 0; q < C; ++q) {
+        left += s.xa[phase][q];
+        most = max(most, s.xa[phase][q]);
+      }
+      phase ^= 1;
+      if (most <= room) {
         // ---- divided by the bits of their keys until few are left
-        kmin = 0;
+        kmin = 1;
         kmax = 0xFFFFFFFFu;
-        uint32_t left = cand;
         while (left > SP_FEW) {
           uint32_t a = 0xFFFFFFFFu, z = 0;
-          for (uint32_t i = tid; i < cand; i += SP_THREADS) {
+          for (int i = tid; i < SP_CAND; i += SP_THREADS) {
             const uint32_t k = s.w.all.key[i];
             if (k >= kmin && k <= kmax) { a = min(a, k); z = max(z, k); }
           }
           a = __reduce_min_sync(0xffffffffu, a);
           z = __reduce_max_sync(0xffffffffu, z);
           if (lane == 0) { s.red[warp] = a; s.red2[warp] = z; }
-          s.w.all.u.sub.cnt[tid] = s.w.all.u.sub.lo[tid] = s.w.all.u.sub.hi[tid] = 0;
+          s.w.all.u.sub.cnt[tid] = s.w.all.u.sub.mass[tid].lo = s.w.all.u.sub.mass[tid].hi = 0;
           __syncthreads();
           for (int w = 0; w < SP_WARPS; ++w) { a = min(a, static_cast<uint32_t>(s.red[w])); z = max(z, static_cast<uint32_t>(s.red2[w])); }
           kmin = a;
           kmax = z;
-          if (kmin == kmax) break;                  // equal logits: ranked by their indices
+          if (kmin == kmax) break;                  // equal logits
           shift = max(0, 32 - __clz(kmax - kmin) - 9);
-          for (uint32_t i = tid; i < cand; i += SP_THREADS) {
+          for (int i = tid; i < SP_CAND; i += SP_THREADS) {
             const uint32_t k = s.w.all.key[i];
             if (k < kmin || k > kmax) continue;
             const int bin = static_cast<int>((kmax - k) >> shift);
@@ -345,70 +359,77 @@ sample_kernel(const SampleParams p) {
             if (by_p) sp_add(s.w.all.u.sub, bin, weight(sp_unkey(k)));
           }
           __syncthreads();
-          const uint32_t here = s.w.all.u.sub.cnt[tid];
-          const int sub = crossing(here, (static_cast<unsigned long long>(s.w.all.u.sub.hi[tid]) << 32) + s.w.all.u.sub.lo[tid], false);
-          left = s.w.all.u.sub.cnt[sub];                  // there is one: the bin passes the limit
+          const int sub = crossing(s.w.all.u.sub.cnt[tid], sp_mass(s.w.all.u.sub, tid), false);
+          left = s.w.all.u.sub.cnt[sub];            // there is one: the bin passes the limit
           const uint32_t high = kmax - (static_cast<uint32_t>(sub) << shift);
           kmin = max(kmin, high - ((1u << shift) - 1));
           kmax = high;
           __syncthreads();                          // sub has been read
         }
-        // ---- ranked
-        if (tid == 0) s.nsel = 0;
-        if (tid < SP_FEW) s.order[tid] = 0;
+        if (tid == 0) { s.nsel = 0; s.found = 0; s.cut_k = 0; s.cut_idx = INT_MAX; }
         __syncthreads();
-        for (uint32_t i = tid; i < cand; i += SP_THREADS) {
-          const uint32_t k = s.w.all.key[i];
-          if (k >= kmin && k <= kmax) {
-            const uint32_t slot = atomicAdd(&s.nsel, 1u);
-            s.h.sel.key[slot] = k;
-            s.h.sel.idx[slot] = s.w.all.idx[i];
+        if (left <= SP_FEW) {
+          // ---- ranked against each other: SP_SEG threads per candidate find its rank and the weights in front of it
+          auto& few = s.w.all.u.few;
+          for (int i = tid; i < SP_CAND; i += SP_THREADS) {
+            const uint32_t k = s.w.all.key[i];
+            if (k >= kmin && k <= kmax) {
+              const uint32_t slot = atomicAdd(&s.nsel, 1u);
+              few.key[slot] = k;
+              few.idx[slot] = s.w.all.idx[i];
+              few.w[slot] = by_p ? weight(sp_unkey(k)) : 0ull;
+            }
           }
-        }
-        __syncthreads();
-        if (left <= SP_FEW) {                       // four threads per candidate
-          constexpr int SEG = SP_THREADS / SP_FEW;
-          const uint32_t i = tid % SP_FEW;
+          __syncthreads();
+          const uint32_t i = tid % SP_FEW, seg = tid / SP_FEW;
+          uint32_t k = 0, d = 0;
           if (i < left) {
-            const uint32_t k = s.h.sel.key[i], d = s.h.sel.idx[i];
+            k = few.key[i];
+            d = few.idx[i];
             uint32_t r = 0;
-            for (uint32_t j = tid / SP_FEW; j < left; j += SEG) r += s.h.sel.key[j] > k || (s.h.sel.key[j] == k && s.h.sel.idx[j] < d);
-            if (r) atomicAdd(&s.order[i], r);
+            unsigned long long sum = 0;
+#pragma unroll 2
+            for (uint32_t j = seg; j < left; j += SP_SEG) {
+              const bool front = few.key[j] > k || (few.key[j] == k && few.idx[j] < d);
+              r += front;
+              sum += front ? few.w[j] : 0ull;
+            }
+            few.rank[seg][i] = r;
+            few.sum[seg][i] = sum;
           }
           __syncthreads();
-          if (tid < left) s.w.all.u.sorted[s.order[tid]] = (static_cast<unsigned long long>(s.h.sel.key[tid]) << 32) | s.h.sel.idx[tid];
+          uint32_t r = 0;
+          unsigned long long run = mass_before;
+          if (tid < left) {
+            for (int q = 0; q < SP_SEG; ++q) { r += few.rank[q][tid]; run += few.sum[q][tid]; }
+            if (by_k && r == top_k - cnt_before - 1) s.cut_k = k;                 // ties with the k-th stay
+            if (by_p && run + few.w[tid] <= limit) atomicMax(&s.found, static_cast<int>(r) + 1);
+          }
+          __syncthreads();
+          if (by_k) cut(s.cut_k, INT_MAX);
+          if (by_p) {
+            const int keep = s.found ? s.found : mass_before == 0 ? 1 : 0;        // the most probable token stays
+            if (tid < left && r == static_cast<uint32_t>(max(keep, 1) - 1)) { s.cut_p = k; s.cut_idx = static_cast<int>(d) - (keep ? 0 : 1); }
+            __syncthreads();
+            cut(s.cut_p, s.cut_idx);
+          }
         } else {
-          for (uint32_t i = tid; i < left; i += SP_THREADS) {
-            const uint32_t k = s.h.sel.key[i], d = s.h.sel.idx[i];
-            uint32_t r = 0;
-            for (uint32_t j = 0; j < left; ++j) r += s.h.sel.key[j] > k || (s.h.sel.key[j] == k && s.h.sel.idx[j] < d);
-            s.w.all.u.sorted[r] = (static_cast<unsigned long long>(k) << 32) | d;
+          // ---- many equal ones: they stay in index order
+          const unsigned long long w = by_p ? weight(sp_unkey(kmin)) : 0ull;
+          unsigned long long keep = left;
+          if (w) keep = limit > mass_before ? min(keep, (limit - mass_before) / w) : 0ull;
+          if (keep == 0 && mass_before == 0) keep = 1;
+          if (keep < left) {
+            if (keep == 0 && tid == 0) s.cut_idx = -1;
+            for (int i = tid; i < SP_CAND; i += SP_THREADS) {
+              if (s.w.all.key[i] != kmin) continue;
+              uint32_t r = 0;
+              for (int j = 0; j < SP_CAND; ++j) r += s.w.all.key[j] == kmin && s.w.all.idx[j] < s.w.all.idx[i];
+              if (r + 1 == keep) s.cut_idx = static_cast<int>(s.w.all.idx[i]);
+            }
           }
-        }
-        __syncthreads();
-        if (by_k) cut(static_cast<uint32_t>(s.w.all.u.sorted[top_k - cnt_before - 1] >> 32), INT_MAX);
-        if (by_p) {                                 // two neighbouring candidates per thread
-          unsigned long long w[2], run;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) w[j] = 2 * tid + j < static_cast<int>(left) ? weight(sp_unkey(static_cast<uint32_t>(s.w.all.u.sorted[2 * tid + j] >> 32))) : 0ull;
-          run = warp_scan64(w[0] + w[1]);
-          if (lane == 31) s.red[warp] = run;
-          if (tid == 0) s.found = 0;
           __syncthreads();
-          run += mass_before - w[0] - w[1];
-          for (int q = 0; q < warp; ++q) run += s.red[q];
-          int keep = 0;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            run += w[j];
-            if (2 * tid + j < static_cast<int>(left) && run <= limit) keep = 2 * tid + j + 1;
-          }
-          if (keep) atomicMax(&s.found, keep);
-          __syncthreads();
-          keep = s.found;
-          const unsigned long long last = s.w.all.u.sorted[max(keep, 1) - 1];
-          if (keep == 0 && mass_before == 0) keep = 1;          // the most probable token stays
-          cut(static_cast<uint32_t>(last >> 32), static_cast<int>(static_cast<uint32_t>(last)) - (keep ? 0 : 1));
+          cut(kmin, s.cut_idx);
         }
         break;
       }
@@ -430,7 +451,7 @@ sample_kernel(const SampleParams p) {
         r->xa[phase][rank] = static_cast<uint32_t>(a2);
         r->xb[phase][rank] = static_cast<uint32_t>(z2);
       }
-      s.h.hist.cnt[tid] = s.h.hist.lo[tid] = s.h.hist.hi[tid] = 0;    // read by all before the barrier in front of the candidates' counts
+      clear();                                      // all have read and are done with the lists of this round
       cluster.sync();
       kmin = 0xFFFFFFFFu;
       kmax = 0;
@@ -443,6 +464,7 @@ sample_kernel(const SampleParams p) {
       }
       // ---- one value: its ties stay in index order
       const unsigned long long w = weight(sp_unkey(kmin));
+      const unsigned long long cand = left;
       unsigned long long keep = cand;
       if (by_p && w) keep = limit > mass_before ? min(keep, (limit - mass_before) / w) : 0ull;
       if (keep == 0 && mass_before == 0) keep = 1;
@@ -459,21 +481,21 @@ sample_kernel(const SampleParams p) {
           cluster.map_shared_rank(&s, tid)->xa[phase][rank] = static_cast<uint32_t>(m);
         }
         cluster.sync();
-        unsigned long long left = keep;             // ties up to and with the last one, from this warp's first on
+        unsigned long long togo = keep;             // ties up to and with the last one, from this warp's first on
         bool here = true;
-        for (int q = 0; q < rank; ++q) { here = here && left > s.xa[phase][q]; left -= s.xa[phase][q]; }
-        for (int q = 0; q < warp; ++q) { here = here && left > s.red[q]; left -= s.red[q]; }
-        if (here && left <= mine) {
+        for (int q = 0; q < rank; ++q) { here = here && togo > s.xa[phase][q]; togo -= s.xa[phase][q]; }
+        for (int q = 0; q < warp; ++q) { here = here && togo > s.red[q]; togo -= s.red[q]; }
+        if (here && togo <= mine) {
           for (int i0 = w0; i0 < w1; i0 += 32) {
             const bool eq = i0 + lane < w1 && sp_key(at(i0 + lane)) == kmin;
             const uint32_t vote = __ballot_sync(0xffffffffu, eq);
             const uint32_t m = __popc(vote);
-            if (left <= m) {
-              if (eq && __popc(vote & ((2u << lane) - 1)) == static_cast<int>(left))
+            if (togo <= m) {
+              if (eq && __popc(vote & ((2u << lane) - 1)) == static_cast<int>(togo))
                 for (int q = 0; q < C; ++q) cluster.map_shared_rank(&s, q)->xb[phase][0] = lo + i0 + lane;
               break;
             }
-            left -= m;
+            togo -= m;
           }
         }
         cluster.sync();
@@ -568,16 +590,16 @@ B200_API int b200_sample(const SampleParams* a, int B, int is_bf16, void* stream
   if (C == 8 && B <= 4 && (p.V + C - 1) / C > 2048) C = 16;        // beyond the portable size, for few rows
   p.per = ((p.V + C - 1) / C + SP_THREADS - 1) / SP_THREADS * SP_THREADS;
   const int smem = (p.per + p.per / 32) * 4;
-  if (smem > 180 * 1024 || static_cast<long long>(B) * C > (1ll << 31) - 1) return -2;
+  if (smem > SP_MAX_SMEM || static_cast<long long>(B) * C > (1ll << 31) - 1) return -2;
   auto kern = is_bf16 ? sample_kernel<__nv_bfloat16> : sample_kernel<float>;
   int dev = 0;
-  static int configured[64][2] = {};
+  static bool configured[64][2] = {};               // the same attributes for every call: threads may set them twice
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
-  if (configured[dev][is_bf16 != 0] < smem) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+  if (!configured[dev][is_bf16 != 0]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_MAX_SMEM) != cudaSuccess ||
         cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return -4;
-    configured[dev][is_bf16 != 0] = smem;
+    configured[dev][is_bf16 != 0] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(B * C));
