@@ -3,6 +3,7 @@
 //   * kv8_rope_append  : the one new token of a decode step from its packed projection: bias, rotation, q out, k and v encoded
 //   * kv8_decode       : codes back to bf16 rows [B, L, Hkv, D] (exact), as the prompt attention reads them
 //   * kv8_tiles        : tile table of the prompt attention, from the lengths on the device
+//   * kv8_nan          : NaNs of V among a prompt's own tokens, put into the rows that see them
 //
 // A block that is begun takes the exponent of its new tokens, so what lay in the cache before does not matter and freed rows need
 // no clearing.  A block that goes on keeps the larger of both exponents; when the new tokens' is larger, what it holds in front of
@@ -100,14 +101,10 @@ kv8_rope_append_kernel(const Kv8Cache c, void* __restrict__ qkv, long long ld, c
   const bool live = unit < c.B * heads && 8 * j < c.D;
   const int b = live ? unit / heads : 0, hh = live ? unit - b * heads : 0;
   const bool rotated = hh < H + c.Hkv;
+  pdl_wait();
   float add[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) add[i] = 0.f;
-  if (live && rotated && bias) {                                    // does not depend on the predecessor
-#pragma unroll
-    for (int i = 0; i < 8; ++i) add[i] = bias[hh * c.D + 8 * j + i];
-  }
-  pdl_wait();
+  for (int i = 0; i < 8; ++i) add[i] = live && rotated && bias ? bias[hh * c.D + 8 * j + i] : 0.f;
   const int p = live ? pos[b] : 0;
   const bool ok = live && p >= 0 && p < c.cap;
   if (live && !ok && err) atomicCAS(err, 0, ERR_BAD_INDEX);
@@ -177,10 +174,11 @@ kv8_rope_append_kernel(const Kv8Cache c, void* __restrict__ qkv, long long ld, c
 }
 
 // out rows [B * L, ld], head h at column h * D: keys (blockIdx.y 0) and values (1) of positions below L.  With `lens`, positions from the
-// length to the next multiple of 128 become zero (an attention tile that ends there reads them) and later ones are left out.
+// length to the next multiple of 128 become zero (an attention tile that ends there reads them) and later ones are left out.  `nan_first`: a weight
+// of zero does not hide a NaN of V from the queries in front of it, so NaNs among the newest n positions become zero and are noted there.
 __global__ void __launch_bounds__(256)
 kv8_decode_kernel(const Kv8Cache c, const int* __restrict__ lens, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
-                  int L, int most, int ld) {
+                  int L, int most, int ld, int* __restrict__ nan_first, int n) {
   pdl_trigger();
   pdl_wait();
   const int vpr = c.D >> 3, per_row = c.Hkv * vpr, b = blockIdx.z;
@@ -193,7 +191,19 @@ kv8_decode_kernel(const Kv8Cache c, const int* __restrict__ lens, __nv_bfloat16*
   if (t < len) {
     const uint8_t* src = (blockIdx.y ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(t) * c.D + d;
     const float f = pow2i((blockIdx.y ? c.ve : c.ke)[b * c.eb + h * c.eh + (t >> c.log2_block)]);
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+    uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+    if (nan_first && blockIdx.y && t >= len - n) {
+      const unsigned long long all = w.x | (static_cast<unsigned long long>(w.y) << 32);
+      unsigned long long keep = ~0ull;
+      if (((all & 0x7F7F7F7F7F7F7F7Full) + 0x0101010101010101ull) & 0x8080808080808080ull)
+        for (int i = 0; i < 8; ++i)
+          if ((all >> (8 * i) & 0x7F) == 0x7F) {
+            keep &= ~(0xFFull << (8 * i));
+            atomicMin(nan_first + (static_cast<long long>(b) * c.Hkv + h) * c.D + d + i, t);
+          }
+      w.x &= static_cast<uint32_t>(keep);
+      w.y &= static_cast<uint32_t>(keep >> 32);
+    }
     const float2 a0 = kv8_float2(w.x, false), a1 = kv8_float2(w.x, true), a2 = kv8_float2(w.y, false), a3 = kv8_float2(w.y, true);
     o = make_uint4(pack_bf16x2(a0.x * f, a0.y * f), pack_bf16x2(a1.x * f, a1.y * f), pack_bf16x2(a2.x * f, a2.y * f), pack_bf16x2(a3.x * f, a3.y * f));
   }
@@ -202,9 +212,10 @@ kv8_decode_kernel(const Kv8Cache c, const int* __restrict__ lens, __nv_bfloat16*
 
 // One CTA per (sequence, 256-query tile): {first query token, queries, stream index of the first query, first key of the sequence}, the tiles
 // that see most keys first.  Queries in front of the sequence's first key have nothing to see: they are not in a tile and their outputs
-// become zero here.
+// become zero here, and the table of NaNs (`noted` entries per sequence) is cleared.
 __global__ void __launch_bounds__(256)
-kv8_tiles_kernel(const int* __restrict__ lens, int4* __restrict__ tiles, __nv_bfloat16* __restrict__ out, int n, int most, int L, int per_seq, long long row) {
+kv8_tiles_kernel(const int* __restrict__ lens, int4* __restrict__ tiles, __nv_bfloat16* __restrict__ out, int n, int most, int L, int per_seq, long long row,
+                 int* __restrict__ nan_first, int noted) {
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.x, i = blockIdx.y, B = gridDim.x;
@@ -215,6 +226,22 @@ kv8_tiles_kernel(const int* __restrict__ lens, int4* __restrict__ tiles, __nv_bf
   uint4* o = reinterpret_cast<uint4*>(out + static_cast<long long>(b) * n * row);
   const long long last = skip * row / 8;
   for (long long x = static_cast<long long>(i) * 256 + threadIdx.x; x < last; x += 256ll * per_seq) o[x] = make_uint4(0u, 0u, 0u, 0u);
+  if (i == 0)
+    for (int x = threadIdx.x; x < noted; x += 256) nan_first[static_cast<long long>(b) * noted + x] = INT_MAX;
+}
+
+// A thread per channel of a key head: the outputs [B, n, H, D] of the queries that see its first noted NaN.
+__global__ void __launch_bounds__(128)
+kv8_nan_kernel(const int* __restrict__ nan_first, const int* __restrict__ lens, __nv_bfloat16* __restrict__ out, int n, int group, int Hkv, int D, int most) {
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.y, h = blockIdx.x, d = threadIdx.x;
+  if (d >= D) return;
+  const int first = nan_first[(static_cast<long long>(b) * Hkv + h) * D + d];
+  if (first == INT_MAX) return;
+  const int len = min(max(lens[b], 0), most);
+  for (int i = max(0, first - (len - n)); i < n; ++i)
+    for (int x = 0; x < group; ++x) out[((static_cast<long long>(b) * n + i) * Hkv * group + h * group + x) * D + d] = __float2bfloat16(NAN);
 }
 
 }  // namespace b200
@@ -269,22 +296,32 @@ B200_API int b200_kv8_rope_append(const Kv8Cache* c, void* qkv, long long ld, in
   return cudaGetLastError() == cudaSuccess ? 0 : -10;
 }
 
-// k_out, v_out: bf16 [B, L, Hkv, D] contiguous, lens: see kv8_decode_kernel (no length counts for more than `most`).
-B200_API int b200_kv8_decode(const Kv8Cache* c, const int* lens, void* k_out, void* v_out, int L, int most, void* stream) {
+// k_out, v_out: bf16 [B, L, Hkv, D] contiguous, lens, nan_first (int32 [B, Hkv, D], cleared; or null), n: see kv8_decode_kernel (no length counts for
+// more than `most`).
+B200_API int b200_kv8_decode(const Kv8Cache* c, const int* lens, void* k_out, void* v_out, int L, int most, int* nan_first, int n, void* stream) {
   if (!kv8_cache_ok(c) || L <= 0 || most > L || most > c->cap || (!lens && L > c->cap)) return -1;
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return -2;
   const long long vecs = static_cast<long long>(L) * c->Hkv * (c->D / 8);
   if (vecs > (1ll << 38)) return -3;
   launch_k(kv8_decode_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256), 2, c->B), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), *c, lens,
-           static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), L, most, c->Hkv * c->D);
+           static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), L, most, c->Hkv * c->D, lens ? nan_first : nullptr, n);
   return cudaGetLastError() == cudaSuccess ? 0 : -10;
 }
 
-// tiles: int4 [B * ceil(n / 256)]; out: bf16 [B, n, row]; most: no length is larger (larger ones are cut), L: key rows per sequence.
-B200_API int b200_kv8_tiles(const int* lens, int* tiles, void* out, int B, int n, int most, int L, long long row, void* stream) {
+// tiles: int4 [B * ceil(n / 256)]; out: bf16 [B, n, row]; most: no length is larger (larger ones are cut), L: key rows per sequence;
+// nan_first: int32 [B, noted].
+B200_API int b200_kv8_tiles(const int* lens, int* tiles, void* out, int B, int n, int most, int L, long long row, int* nan_first, int noted, void* stream) {
   const int per_seq = (n + 255) / 256;
   if (B <= 0 || n <= 0 || per_seq > 65535 || most > L || (row & 7)) return -1;
   launch_k(kv8_tiles_kernel, dim3(B, per_seq), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), lens, reinterpret_cast<int4*>(tiles),
-           static_cast<__nv_bfloat16*>(out), n, most, L, per_seq, row);
+           static_cast<__nv_bfloat16*>(out), n, most, L, per_seq, row, nan_first, noted);
+  return cudaGetLastError() == cudaSuccess ? 0 : -10;
+}
+
+// nan_first: as kv8_decode noted it; out: bf16 [B, n, Hkv * group, D].
+B200_API int b200_kv8_nan(const int* nan_first, const int* lens, void* out, int B, int n, int group, int Hkv, int D, int most, void* stream) {
+  if (B <= 0 || B > 65535 || n <= 0 || group <= 0 || Hkv <= 0 || D <= 0 || D > 128) return -1;
+  launch_k(kv8_nan_kernel, dim3(Hkv, B), dim3(128), 0, reinterpret_cast<cudaStream_t>(stream), nan_first, lens, static_cast<__nv_bfloat16*>(out), n, group, Hkv,
+           D, most);
   return cudaGetLastError() == cudaSuccess ? 0 : -10;
 }

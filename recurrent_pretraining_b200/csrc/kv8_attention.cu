@@ -14,8 +14,9 @@
 // times 2^15: eleven significant bits for every contribution down to 2^-29 of the largest.
 //
 // Scales are powers of two: K's enters the score, V's the exponent of the weight, so that the running reference R = max(s + e_v)
-// belongs to the contributions to O.  The sum of the weights counts from e_ref, the exponent of the sequence's first block of values:
-//   O = sum 2^(s + e_v - R) code_v,  l = sum 2^(s + e_v - R) 2^(e_ref - e_v),  o = O / l * 2^e_ref.
+// belongs to the contributions to O.  The sum of the weights counts from the middle of the exponents' range, E = 40:
+//   O = sum 2^(s + e_v - R) code_v,  l = sum 2^(s + e_v - R) 2^(E - e_v),  o = O / l * 2^E,
+// so that its terms stay below 2^95 and none that counts is lost below 2^-126, however far apart the exponents of two blocks are.
 // Scores, references, sums and accumulators are fp32.
 //
 // Work is split evenly whatever the lengths are: the keys of all (sequence, key head, row tile) ranges lie one behind the other in steps of 32,
@@ -46,6 +47,7 @@ struct Kv8Attn {
 };
 
 constexpr int KA_WARPS = 4, KA_STEP = 32;           // keys per warp and step
+constexpr int KA_MID = 40;                          // E above
 constexpr float KA_NEG = -1.5e38f;                  // "no key yet": finite, so that differences stay defined
 
 // c += a b, a f16 [16 x 16], b f16 [16 x 8]
@@ -260,9 +262,9 @@ kv8_attention_kernel(const Kv8Attn p) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // What a range begins with is loaded while the one before it is worked on: q rows (lane g: row g of a column tile), exponents of the first
-  // step and of the sequence's first block of values.
+  // step.
   uint2 q_raw[NT == 1 ? 2 * KS : 1];
-  int kex[2] = {0, 0}, vex[2] = {0, 0}, e_ref = 0;
+  int kex[2] = {0, 0}, vex[2] = {0, 0};
   auto exponents = [&](const Range& r, int at) {
     const int8_t *kep = p.ke + r.b * p.eb + r.h * p.eh, *vep = p.ve + r.b * p.eb + r.h * p.eh;
     const int e0 = min(at, r.key1 - 1) >> p.log2_block, e1 = min(at + 16, r.key1 - 1) >> p.log2_block;
@@ -304,7 +306,7 @@ kv8_attention_kernel(const Kv8Attn p) {
     }
     return pow2i(e) * p.scale_log2;
   };
-  int first_e[5];
+  int first_e[4];
   auto prepare = [&](const Range& r) {
     if constexpr (NT == 1) q_load(r, 0, q_raw);
     if (r.key1 > r.key0) {
@@ -314,7 +316,6 @@ kv8_attention_kernel(const Kv8Attn p) {
       first_e[1] = __ldg(kep + e1);
       first_e[2] = __ldg(vep + e0);
       first_e[3] = __ldg(vep + e1);
-      first_e[4] = __ldg(vep);
     }
   };
   nxt.next(p, sh, hi);
@@ -356,7 +357,7 @@ kv8_attention_kernel(const Kv8Attn p) {
       }
     }
     kex[0] = first_e[0]; kex[1] = first_e[1]; vex[0] = first_e[2]; vex[1] = first_e[3];
-    e_ref = key1 > now.key0 ? first_e[4] : 0;
+    int vmax = KV8_EMIN;                            // largest exponent of V so far
     more = nxt.step < hi;
     if (more) {
       nxt.next(p, sh, hi);
@@ -421,7 +422,9 @@ kv8_attention_kernel(const Kv8Attn p) {
         for (int w = 0; w < VB; ++w) ldmatrix2_trans8(v[w], here + Ring::TILE + ((v_row + 16 * w) ^ v_twist));
       }
       const float kf[2] = {pow2i(kex[0]), pow2i(kex[1])}, vf[2] = {static_cast<float>(vex[0]), static_cast<float>(vex[1])};
-      const float cf[2] = {pow2i(min(e_ref - vex[0], 127)), pow2i(min(e_ref - vex[1], 127))};
+      const float cf[2] = {pow2i(KA_MID - vex[0]), pow2i(KA_MID - vex[1])};
+      vmax = max(vmax, max(vex[0], vex[1]));
+      const bool apart = vmax - min(vex[0], vex[1]) > 64;       // weights that O cannot hold may count in l (all lanes alike)
       exponents(now, key + KA_STEP);
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -453,9 +456,9 @@ kv8_attention_kernel(const Kv8Attn p) {
             for (int i = 0; i < 2; ++i) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], x));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float rn = fmaxf(R[c8][i], mx[i]), alpha = ex2_approx(R[c8][i] - rn);
+            const float rn = fmaxf(R[c8][i], mx[i]), half = ex2_approx(0.5f * (R[c8][i] - rn)), alpha = half * half;
             R[c8][i] = rn;
-            l[c8][i] *= alpha;
+            l[c8][i] = l[c8][i] * half * half;      // alpha may be too small for a number where this is not
 #pragma unroll
             for (int w = 0; w < VB; ++w) {
               o[w][c8][i] *= alpha;
@@ -470,7 +473,8 @@ kv8_attention_kernel(const Kv8Attn p) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             w4[i] = ex2_approx(s[m][c8][i] - up[i & 1]);
-            l[c8][i & 1] = fmaf(w4[i], cf[m], l[c8][i & 1]);
+            if (!apart) l[c8][i & 1] = fmaf(w4[i], cf[m], l[c8][i & 1]);
+            else l[c8][i & 1] += ex2_approx(s[m][c8][i] - up[i & 1] - vf[m] + KA_MID);
           }
           pb[c8][2 * m] = transpose8x8(half2_bits(w4[0], w4[1]));
           pb[c8][2 * m + 1] = transpose8x8(half2_bits(w4[2], w4[3]));
@@ -530,12 +534,12 @@ kv8_attention_kernel(const Kv8Attn p) {
             }
           }
           if (whole) {
-            const float f = sum == 0.f ? 0.f : 1.f / sum, e = pow2i(e_ref);
+            const float f = sum == 0.f ? 0.f : 1.f / sum, e = pow2i(KA_MID);
             __nv_bfloat16* to = p.out + ((static_cast<size_t>(now.b) * p.n + tok) * p.Hkv * p.group + hq) * D + g;
 #pragma unroll
             for (int w = 0; w < VB; ++w) {
-              to[16 * w] = f2bf(o[w][c8][i] * f * e);
-              to[16 * w + 8] = f2bf(o[w][c8][i + 2] * f * e);
+              to[16 * w] = f2bf(o[w][c8][i] * e * f);
+              to[16 * w + 8] = f2bf(o[w][c8][i + 2] * e * f);
             }
           } else {
             float* to = p.part + ((2ll * worker + (now.begins ? 1 : 0)) * p.rows + c) * (D + 4) + g;
@@ -571,7 +575,6 @@ kv8_join_kernel(const Kv8Attn p) {
   const int h = unit / p.tiles_r, row = (unit - h * p.tiles_r) * p.rows + r;
   const bool mine = n > 1 && unit < static_cast<int>(sh.per_unit) && row < p.n * p.group;
   const int c0 = mine ? sh.owner(base + unit * n) : 0, parts = mine ? sh.owner(base + unit * n + n - 1) - c0 + 1 : 1;
-  const float e = pow2i(mine ? p.ve[b * p.eb + h * p.eh] : 0);
   pdl_trigger();
   pdl_wait();
   if (WR >= 4 && parts == 1) return;                // written by its warp
@@ -597,14 +600,15 @@ kv8_join_kernel(const Kv8Attn p) {
 #pragma unroll
     for (int i = 0; i < ML; ++i) tn = fmaxf(tn, ml[i].x);
     tn = warp_max(tn);
-    const float f0 = ex2_approx(top - tn);
+    const float f0h = ex2_approx(0.5f * (top - tn)), f0 = f0h * f0h;
     top = tn;
 #pragma unroll
     for (int i = 0; i < ML; ++i) {
-      ml[i].x = ex2_approx(ml[i].x - tn);
-      s += ml[i].y * ml[i].x;
+      const float half = ex2_approx(0.5f * (ml[i].x - tn));     // twice, as above
+      ml[i].x = half * half;
+      s += ml[i].y * half * half;
     }
-    sum = sum * f0 + warp_sum(s);
+    sum = sum * f0h * f0h + warp_sum(s);
     acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {             // part WR i + place: lane (WR i + place) % 32 of round (WR i + place) / 32
@@ -623,10 +627,10 @@ kv8_join_kernel(const Kv8Attn p) {
     }
   }
   if (parts == 1 || lane >= D / 4) return;
-  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  const float f = sum == 0.f ? 0.f : 1.f / sum, e = pow2i(KA_MID);
   const int i = row / p.group, hq = h * p.group + row - i * p.group;
   *reinterpret_cast<uint2*>(p.out + ((static_cast<size_t>(b) * p.n + i) * p.Hkv * p.group + hq) * D + 4 * lane) =
-      make_uint2(pack_bf16x2(acc.x * f * e, acc.y * f * e), pack_bf16x2(acc.z * f * e, acc.w * f * e));
+      make_uint2(pack_bf16x2(acc.x * e * f, acc.y * e * f), pack_bf16x2(acc.z * e * f, acc.w * e * f));
 }
 
 template <int D, int NT>

@@ -8,9 +8,9 @@ capacity / block]``; a value is ``code * 2**exponent``.  The exponent of a block
 first position is written, so rows of an earlier sequence need no clearing; a sequence is written in order, and writing at a position
 again forgets what lies behind it in the block.  Infinities are stored as the block's largest code, NaN as NaN.
 
-Sequences are described by int32 tensors on the cache's device and never read by the host: a position or length outside the cache is
-left out by the kernels (nothing is written; lengths are cut to the capacity) and recorded in the device status word
-(``cuda.check_device_status``).  Calls run on the current stream and allocate through PyTorch's allocator."""
+Sequences are described by int32 tensors on the cache's device and never read by the host: positions outside the cache are left out by
+the kernels (nothing is written) and recorded in the device status word (``cuda.check_device_status``), lengths are cut to the capacity.
+Calls run on the current stream and allocate through PyTorch's allocator."""
 from __future__ import annotations
 
 import ctypes as C
@@ -53,8 +53,9 @@ def _k():
             K=K, check=K._check, stream=K._stream,
             append=K._sig("b200_kv8_append", [C.POINTER(_Cache), vp, vp, C.POINTER(ll), vp, vp, i, vp, vp]),
             rope=K._sig("b200_kv8_rope_append", [C.POINTER(_Cache), vp, ll, i, i, vp, vp, vp, vp, vp, i, vp, vp]),
-            decode=K._sig("b200_kv8_decode", [C.POINTER(_Cache), vp, vp, vp, i, i, vp]),
-            tiles=K._sig("b200_kv8_tiles", [vp, vp, vp, i, i, i, i, ll, vp]),
+            decode=K._sig("b200_kv8_decode", [C.POINTER(_Cache), vp, vp, vp, i, i, vp, i, vp]),
+            tiles=K._sig("b200_kv8_tiles", [vp, vp, vp, i, i, i, i, ll, vp, i, vp]),
+            nan=K._sig("b200_kv8_nan", [vp] * 3 + [i] * 6 + [vp]),
             plan=K._sig("b200_kv8_attention_plan", [i] * 5 + [C.POINTER(i)]),
             attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn)] + [vp] * 5),
             long_ok=K._sig("b200_capped_attention_supported", [i, i]),
@@ -131,7 +132,7 @@ class KV8Cache:
             return tuple(ref.kv8_decode(c, e).transpose(1, 2).to(BF16) for c, e in ((self.k, self.k_exp), (self.v, self.v_exp)))
         k, v = (torch.empty(self.batch, self.capacity, self.kv_heads, self.dim, dtype=BF16, device=self.device) for _ in range(2))
         f = _k()
-        _guarded(self.device, lambda: f.K._check(f.decode(C.byref(self._c), 0, k.data_ptr(), v.data_ptr(), self.capacity, self.capacity, f.K._stream()),
+        _guarded(self.device, lambda: f.K._check(f.decode(C.byref(self._c), 0, k.data_ptr(), v.data_ptr(), self.capacity, self.capacity, 0, 0, f.K._stream()),
                                                  "kv8_decode"))
         return k, v
 
@@ -330,10 +331,12 @@ def _long(q, cache, lens, scale, most) -> torch.Tensor:
         out = torch.empty(B, n, H, D, dtype=BF16, device=cache.device)
         kv = torch.empty(2, B * L, W, dtype=BF16, device=cache.device)
         tiles = torch.empty(B * per, 4, dtype=torch.int32, device=cache.device)
-        K._check(f.decode(C.byref(cache._c), lens.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), L, most, st), "kv8_decode")
-        K._check(f.tiles(lens.data_ptr(), tiles.data_ptr(), out.data_ptr(), B, n, most, L, H * D, st), "kv8_tiles")
+        nans = torch.empty(B, W, dtype=torch.int32, device=cache.device)
+        K._check(f.tiles(lens.data_ptr(), tiles.data_ptr(), out.data_ptr(), B, n, most, L, H * D, nans.data_ptr(), W, st), "kv8_tiles")
+        K._check(f.decode(C.byref(cache._c), lens.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), L, most, nans.data_ptr(), n, st), "kv8_decode")
         K._check(f.long(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), 0, B * per, B * n, B * L, H, Hkv, D, D,
                         H * D, W, H * D, 2 ** 30, 0, scale, 0.0, 0.0, st, K.err_word(cache.device).data_ptr()), "capped_attention")
+        K._check(f.nan(nans.data_ptr(), lens.data_ptr(), out.data_ptr(), B, n, H // Hkv, Hkv, D, most, st), "kv8_nan")
         return out
 
     return _guarded(cache.device, run)

@@ -80,9 +80,12 @@ def test_a_prompt_in_two_chunks_reads_the_decoded_cache(model):
 @gpu
 @pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
 def test_sampled_tokens(model, kv_dtype):
-    """Sampling is what ``sample_tokens`` draws from the engine's own logits; a generator repeats it, and the narrowest filters are greedy."""
+    """Sampling is what ``sample_tokens`` draws from the engine's own logits with the generator's numbers, and the narrowest filters are
+    greedy.  (The logits of two runs may differ in their last bits, since the products of a step add their parts atomically, so equal
+    numbers need not give equal tokens.)"""
     from recurrent_pretraining_b200.engine.decode import DecodeEngine
     from recurrent_pretraining_b200.models.sampling import SamplingOptions
+    from recurrent_pretraining_b200.ops.sampling import sample_tokens
 
     ids = torch.randint(0, 4000, (2, 20), device="cuda", generator=torch.Generator("cuda").manual_seed(5))
     eng = DecodeEngine(model, max_batch=2, max_len=64, num_steps=4, kv_dtype=kv_dtype)
@@ -90,8 +93,12 @@ def test_sampled_tokens(model, kv_dtype):
                                          generator=torch.Generator("cuda").manual_seed(seed))[0]
     greedy = eng.generate(ids, 10, init_scale=0.0)[0]
     assert torch.equal(run(1, top_k=1), greedy) and torch.equal(run(2, top_p=1e-9), greedy) and torch.equal(run(3, min_p=1.0), greedy)
-    a = run(7, temperature=1.5, top_k=200, top_p=0.95)
-    assert torch.equal(a, run(7, temperature=1.5, top_k=200, top_p=0.95)) and not torch.equal(a, run(8, temperature=1.5, top_k=200, top_p=0.95))
+    assert not torch.equal(run(7, temperature=1.5, top_k=200, top_p=0.95), run(8, temperature=1.5, top_k=200, top_p=0.95))
+    logits = torch.randn(2, 4096, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    numbers = torch.rand(2, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    options = dict(temperature=1.5, top_k=200, top_p=0.95)
+    eng.uniform[:2] = numbers
+    assert torch.equal(eng._pick(logits, eng._settings(SamplingOptions(do_sample=True, **options))), sample_tokens(logits, numbers, **options))
     assert torch.equal(eng.generate(ids, 10, init_scale=0.0, sampling=SamplingOptions(temperature=3.0))[0], greedy)      # do_sample is off
     with pytest.raises(ValueError):
         eng.generate(ids, 4, criterion="kl", sampling=SamplingOptions(do_sample=True))

@@ -360,6 +360,47 @@ def test_attention_nan_reaches_only_those_who_see_it(device):
     assert torch.equal(out[~out.isnan()], clean[~out.isnan()])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_long_attention_nan_reaches_only_those_who_see_it(device):
+    B, n, H, Hkv, D, cap = 2, 70, 4, 2, 64, 416
+    cache = filled(B, Hkv, cap, D, 32, device)
+    q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(device)
+    lens = i32([400, 75], device)
+    clean = kv8.attention(q, cache, lens)
+    v, k = cache.v.view(torch.uint8), cache.k.view(torch.uint8)
+    v[0, 0, 390, 5] = v[0, 0, 395, 5] = 0x7F                # seen by the last ten tokens
+    v[0, 0, 20, 6] = 0xFF                                   # by all
+    k[0, 1, 399, 9] = 0xFF                                  # by the last one
+    v[1, 1, 74, 0] = v[1, 1, 5, 1] = 0x7F                   # by the last one; by all
+    out = kv8.attention(q, cache, lens)
+    nan = torch.zeros(B, n, H, D, dtype=torch.bool)
+    nan[0, 60:, :2, 5] = nan[0, :, :2, 6] = nan[0, 69, 2:] = nan[1, 69, 2:, 0] = nan[1, :, 2:, 1] = True
+    assert torch.equal(out.isnan().cpu(), nan)
+    assert torch.equal(out[~out.isnan()], clean[~out.isnan()])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n,group", [(1, 1), (3, 2)])
+@pytest.mark.parametrize("order", ["small first", "large first"])
+def test_attention_with_exponents_at_both_ends(device, n, group, order):
+    """A block of the largest values next to blocks of the smallest: every key counts in the sum of the weights."""
+    B, Hkv, D, block, cap = 2, 2, 64, 16, 640
+    g = torch.Generator().manual_seed(11)
+    cache = KV8Cache.empty(B, Hkv, cap, D, device, block)
+    k, v = (torch.randn(B, cap, Hkv, D, generator=g) for _ in range(2))
+    v = v.clamp(0.1, 3.0) * 2.0 ** -45
+    at = 0 if order == "large first" else 320
+    v[:, at:at + block] = v[:, at:at + block] * 2.0 ** 45 * 2.0 ** 124
+    kv8.append(cache, k.to(torch.bfloat16).to(device), v.to(torch.bfloat16).to(device), i32([0] * B, device))
+    assert cache.v_exp.max() > 115 and cache.v_exp.min() == -40
+    q = torch.randn(B, n, Hkv * group, D, generator=g).to(torch.bfloat16)
+    lens = [cap, 330]
+    out = kv8.attention(q.to(device), cache, i32(lens, device)).double().cpu()
+    want, mag, big = attend(q.double(), values(cache, "k"), values(cache, "v"), lens, D ** -0.5)
+    tol = tolerance(want, mag, big, D, F16_HALF)
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() / tol).max()
+
+
 def test_refusals():
     cache = KV8Cache.empty(2, 2, 64, 32)
     k, p = torch.zeros(2, 4, 2, 32, dtype=torch.bfloat16), i32([0, 0], "cpu")
