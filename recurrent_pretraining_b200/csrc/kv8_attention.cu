@@ -11,7 +11,8 @@
 // have to be split into 8-bit parts, four products each, and a tile's maximum and weights go through barriers of the whole CTA.)
 //
 // q enters as f16 under a power of two per row, which keeps bf16's eight bits down to 2^-28 of the row's largest.  Weights enter as f16
-// times 2^15: eleven significant bits for every contribution down to 2^-29 of the largest.
+// times 2^12, and the reference moves only when a score exceeds it by more than 3 (log2 units; most steps of short shares would move
+// it otherwise): eleven significant bits for every contribution down to 2^-26 of the largest.
 //
 // Scales are powers of two: K's enters the score, V's the exponent of the weight, so that the running reference R = max(s + e_v)
 // belongs to the contributions to O.  The sum of the weights counts from the middle of the exponents' range, E = 40:
@@ -48,6 +49,7 @@ struct Kv8Attn {
 
 constexpr int KA_WARPS = 4, KA_STEP = 32;           // keys per warp and step
 constexpr int KA_MID = 40;                          // E above
+constexpr float KA_UP = 12.f, KA_SLACK = 3.f;       // weights reach 2^15
 constexpr float KA_NEG = -1.5e38f;                  // "no key yet": finite, so that differences stay defined
 
 // c += a b, a f16 [16 x 16], b f16 [16 x 8]
@@ -422,9 +424,9 @@ kv8_attention_kernel(const Kv8Attn p) {
         for (int w = 0; w < VB; ++w) ldmatrix2_trans8(v[w], here + Ring::TILE + ((v_row + 16 * w) ^ v_twist));
       }
       const float kf[2] = {pow2i(kex[0]), pow2i(kex[1])}, vf[2] = {static_cast<float>(vex[0]), static_cast<float>(vex[1])};
-      const float cf[2] = {pow2i(KA_MID - vex[0]), pow2i(KA_MID - vex[1])};
       vmax = max(vmax, max(vex[0], vex[1]));
-      const bool apart = vmax - min(vex[0], vex[1]) > 64;       // weights that O cannot hold may count in l (all lanes alike)
+      const bool apart = vmax - min(vex[0], vex[1]) > 64;       // weights that are no numbers for O may count in l (all lanes alike)
+      const float cf[2] = {apart ? 0.f : pow2i(KA_MID - vex[0]), apart ? 0.f : pow2i(KA_MID - vex[1])};
       exponents(now, key + KA_STEP);
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -449,7 +451,7 @@ kv8_attention_kernel(const Kv8Attn p) {
         float mx[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) mx[i] = fmaxf(fmaxf(s[0][c8][i], s[0][c8][i + 2]), fmaxf(s[1][c8][i], s[1][c8][i + 2]));
-        if (__any_sync(0xffffffffu, mx[0] > R[c8][0] || mx[1] > R[c8][1])) {    // seldom after the first steps
+        if (__any_sync(0xffffffffu, mx[0] > R[c8][0] + KA_SLACK || mx[1] > R[c8][1] + KA_SLACK)) {    // seldom after the first step
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1)
 #pragma unroll
@@ -466,15 +468,20 @@ kv8_attention_kernel(const Kv8Attn p) {
             }
           }
         }
-        const float up[2] = {R[c8][0] - 15.f, R[c8][1] - 15.f};
+        const float up[2] = {R[c8][0] - KA_UP, R[c8][1] - KA_UP};
+        if (apart) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[c8][i & 1] += ex2_approx(s[m][c8][i] - up[i & 1] - vf[m] + KA_MID);
+        }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           float w4[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             w4[i] = ex2_approx(s[m][c8][i] - up[i & 1]);
-            if (!apart) l[c8][i & 1] = fmaf(w4[i], cf[m], l[c8][i & 1]);
-            else l[c8][i & 1] += ex2_approx(s[m][c8][i] - up[i & 1] - vf[m] + KA_MID);
+            l[c8][i & 1] = fmaf(w4[i], cf[m], l[c8][i & 1]);
           }
           pb[c8][2 * m] = transpose8x8(half2_bits(w4[0], w4[1]));
           pb[c8][2 * m + 1] = transpose8x8(half2_bits(w4[2], w4[3]));
