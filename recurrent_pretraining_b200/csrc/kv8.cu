@@ -20,33 +20,39 @@ struct Kv8Cache {
   int B, Hkv, cap, D, log2_block;
 };
 
-// grid (2 x most touched blocks, Hkv, B), 128 threads.  The block's new tokens stay in registers (NV vectors of eight values per
-// thread) between the maximum and the encoding: one pass over the input.
-template <int NV>
+// Values of a block up to which a warp takes it (4 x 1024 tokens of 55 heads of 96 in blocks of 32: 28.0 us with 128 threads to a block, 30.3 with a
+// warp; 13 x 77 tokens of 8 heads of 128: 3.0 and 4.1 us).
+constexpr int KV8_WARP_VALUES = 1024;
+
+// grid (2 x most touched blocks / (128 / G), Hkv, B), 128 threads, G of them (a warp or the CTA) per block of BLK tokens.  The block's new tokens
+// stay in registers (NV vectors of eight values per thread) between the maximum and the encoding: one pass over the input.  D and BLK
+// are known to the compiler: a division per vector would take longer than the vector.
+template <int D, int BLK, int G>
 __global__ void __launch_bounds__(128)
 kv8_append_kernel(const Kv8Cache c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long k_sb,
                   long long k_sn, long long k_sh, long long v_sb, long long v_sn, long long v_sh, const int* __restrict__ start_,
                   const int* __restrict__ counts, int n, int* err) {
   pdl_trigger();
   pdl_wait();
-  const int which = blockIdx.x & 1, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int unit = blockIdx.x * (128 / G) + threadIdx.x / G, which = unit & 1, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x % G;
   const int start = start_[b], cnt = counts ? counts[b] : n;
   if (start < 0 || cnt < 0 || cnt > n || start > c.cap - cnt) {     // the sequence does not fit: nothing of it is written
     if (tid == 0 && err) atomicCAS(err, 0, ERR_BAD_INDEX);
     return;
   }
-  const int block = (start >> c.log2_block) + (blockIdx.x >> 1), p0 = block << c.log2_block;
-  const int lo = max(start, p0), hi = min(start + cnt, p0 + (1 << c.log2_block));
+  const int block = start / BLK + (unit >> 1), p0 = block * BLK;
+  const int lo = max(start, p0), hi = min(start + cnt, p0 + BLK);
   if (lo >= hi) return;
   const long long sn = which ? v_sn : k_sn;
   const __nv_bfloat16* src = (which ? v + b * v_sb + h * v_sh : k + b * k_sb + h * k_sh) + (lo - start) * sn;
-  uint8_t* dst = (which ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(p0) * c.D;
+  uint8_t* dst = (which ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(p0) * D;
   int8_t* ep = (which ? c.ve : c.ke) + b * c.eb + h * c.eh + block;
-  const int vpr = c.D >> 3, nvec = (hi - lo) * vpr;
+  constexpr int vpr = D / 8, NV = (BLK * vpr + G - 1) / G;
+  const int nvec = (hi - lo) * vpr;
   uint4 x[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int idx = tid + 128 * i;
+    const int idx = tid + G * i;
     x[i] = make_uint4(0u, 0u, 0u, 0u);
     if (idx < nvec) x[i] = __ldg(reinterpret_cast<const uint4*>(src + (idx / vpr) * sn) + idx % vpr);
   }
@@ -62,26 +68,28 @@ kv8_append_kernel(const Kv8Cache c, const __nv_bfloat16* __restrict__ k, const _
       amax = fmaxf(amax, fmaxf(kv8_mag(f.x), kv8_mag(f.y)));
     }
   }
-  __shared__ float red[4];
-  amax = warp_max(amax);
-  if ((tid & 31) == 0) red[tid >> 5] = amax;
-  __syncthreads();                                                  // every thread has read the old exponent, too
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  amax = warp_max(amax);                                            // every thread has read the old exponent, too
+  if constexpr (G > 32) {
+    __shared__ float red[4];
+    if ((tid & 31) == 0) red[tid >> 5] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
   const int e = max(kv8_exponent(amax), old);
   const float inv = pow2i(-e);
   if (tid == 0) *ep = static_cast<int8_t>(e);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int idx = tid + 128 * i;
+    const int idx = tid + G * i;
     if (idx < nvec) {
       const float2 f0 = unpack_bf16x2(x[i].x), f1 = unpack_bf16x2(x[i].y), f2 = unpack_bf16x2(x[i].z), f3 = unpack_bf16x2(x[i].w);
-      *reinterpret_cast<uint2*>(dst + static_cast<size_t>(lo - p0) * c.D + 8 * static_cast<size_t>(idx)) =
+      *reinterpret_cast<uint2*>(dst + static_cast<size_t>(lo - p0) * D + 8 * static_cast<size_t>(idx)) =
           make_uint2(kv8_encode4(f0.x, f0.y, f1.x, f1.y, inv), kv8_encode4(f2.x, f2.y, f3.x, f3.y, inv));
     }
   }
   if (!fresh && e > old) {
     const float f = pow2i(old - e);
-    for (int idx = tid; idx < (lo - p0) * vpr; idx += 128) {
+    for (int idx = tid; idx < (lo - p0) * vpr; idx += G) {
       uint2* w = reinterpret_cast<uint2*>(dst) + idx;
       *w = make_uint2(kv8_recode4(w->x, f), kv8_recode4(w->y, f));
     }
@@ -183,31 +191,36 @@ kv8_decode_kernel(const Kv8Cache c, const int* __restrict__ lens, __nv_bfloat16*
   pdl_wait();
   const int vpr = c.D >> 3, per_row = c.Hkv * vpr, b = blockIdx.z;
   const long long idx = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const int t = static_cast<int>(idx / per_row), col = static_cast<int>(idx - static_cast<long long>(t) * per_row);
+  const int t0 = 4 * static_cast<int>(idx / per_row), col = static_cast<int>(idx - static_cast<long long>(t0 / 4) * per_row);   // tokens t0 .. t0 + 3, eight channels
   const int len = lens ? min(max(lens[b], 0), most) : L;
-  if (t >= min(L, (len + 127) & ~127)) return;
+  const int end = min(L, (len + 127) & ~127);
+  if (t0 >= end) return;
   const int h = col / vpr, d = (col - h * vpr) * 8;
-  uint4 o = make_uint4(0u, 0u, 0u, 0u);
-  if (t < len) {
-    const uint8_t* src = (blockIdx.y ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(t) * c.D + d;
-    const float f = pow2i((blockIdx.y ? c.ve : c.ke)[b * c.eb + h * c.eh + (t >> c.log2_block)]);
-    uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-    if (nan_first && blockIdx.y && t >= len - n) {
-      const unsigned long long all = w.x | (static_cast<unsigned long long>(w.y) << 32);
+  const uint8_t* src = (blockIdx.y ? c.v : c.k) + b * c.sb + h * c.sh + static_cast<long long>(t0) * c.D + d;
+  __nv_bfloat16* dst = (blockIdx.y ? v_out : k_out) + (static_cast<long long>(b) * L + t0) * ld + h * c.D + d;
+  uint2 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = t0 + i < len ? __ldg(reinterpret_cast<const uint2*>(src + i * c.D)) : make_uint2(0u, 0u);
+  const float f = t0 < len ? pow2i((blockIdx.y ? c.ve : c.ke)[b * c.eb + h * c.eh + (t0 >> c.log2_block)]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (t0 + i >= end) break;
+    if (nan_first && blockIdx.y && t0 + i >= len - n) {
+      const unsigned long long all = w[i].x | (static_cast<unsigned long long>(w[i].y) << 32);
       unsigned long long keep = ~0ull;
       if (((all & 0x7F7F7F7F7F7F7F7Full) + 0x0101010101010101ull) & 0x8080808080808080ull)
-        for (int i = 0; i < 8; ++i)
-          if ((all >> (8 * i) & 0x7F) == 0x7F) {
-            keep &= ~(0xFFull << (8 * i));
-            atomicMin(nan_first + (static_cast<long long>(b) * c.Hkv + h) * c.D + d + i, t);
+        for (int x = 0; x < 8; ++x)
+          if ((all >> (8 * x) & 0x7F) == 0x7F) {
+            keep &= ~(0xFFull << (8 * x));
+            atomicMin(nan_first + (static_cast<long long>(b) * c.Hkv + h) * c.D + d + x, t0 + i);
           }
-      w.x &= static_cast<uint32_t>(keep);
-      w.y &= static_cast<uint32_t>(keep >> 32);
+      w[i].x &= static_cast<uint32_t>(keep);
+      w[i].y &= static_cast<uint32_t>(keep >> 32);
     }
-    const float2 a0 = kv8_float2(w.x, false), a1 = kv8_float2(w.x, true), a2 = kv8_float2(w.y, false), a3 = kv8_float2(w.y, true);
-    o = make_uint4(pack_bf16x2(a0.x * f, a0.y * f), pack_bf16x2(a1.x * f, a1.y * f), pack_bf16x2(a2.x * f, a2.y * f), pack_bf16x2(a3.x * f, a3.y * f));
+    const float2 a0 = kv8_float2(w[i].x, false), a1 = kv8_float2(w[i].x, true), a2 = kv8_float2(w[i].y, false), a3 = kv8_float2(w[i].y, true);
+    *reinterpret_cast<uint4*>(dst + static_cast<long long>(i) * ld) =
+        make_uint4(pack_bf16x2(a0.x * f, a0.y * f), pack_bf16x2(a1.x * f, a1.y * f), pack_bf16x2(a2.x * f, a2.y * f), pack_bf16x2(a3.x * f, a3.y * f));
   }
-  *reinterpret_cast<uint4*>((blockIdx.y ? v_out : k_out) + (static_cast<long long>(b) * L + t) * ld + h * c.D + d) = o;
 }
 
 // One CTA per (sequence, 256-query tile): {first query token, queries, stream index of the first query, first key of the sequence}, the tiles
@@ -263,19 +276,21 @@ B200_API int b200_kv8_append(const Kv8Cache* c, const void* k, const void* v, co
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
   const int blk = 1 << c->log2_block;
   const long long touched = (static_cast<long long>(n) + blk - 2) / blk + 1;
-  const dim3 grid(static_cast<unsigned>(2 * touched), c->Hkv, c->B);
-  const int nv = (blk * (c->D / 8) + 127) / 128;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const __nv_bfloat16 *kb = static_cast<const __nv_bfloat16*>(k), *vb = static_cast<const __nv_bfloat16*>(v);
-#define RUN(NV) launch_k(kv8_append_kernel<NV>, grid, dim3(128), 0, st, *c, kb, vb, pitch[0], pitch[1], pitch[2], pitch[3], pitch[4], pitch[5], start, counts, n, err)
-  if (nv == 1) RUN(1);
-  else if (nv == 2) RUN(2);
-  else if (nv == 3) RUN(3);
-  else if (nv == 4) RUN(4);
-  else if (nv <= 6) RUN(6);
-  else if (nv <= 8) RUN(8);
-  else if (nv <= 12) RUN(12);
-  else RUN(16);
+#define RUN(D, BLK) \
+  case D * 1000 + BLK: { \
+    constexpr int G = BLK * D <= KV8_WARP_VALUES ? 32 : 128; \
+    launch_k(kv8_append_kernel<D, BLK, G>, dim3(static_cast<unsigned>((2 * touched + 128 / G - 1) / (128 / G)), c->Hkv, c->B), dim3(128), 0, st, *c, kb, vb, \
+             pitch[0], pitch[1], pitch[2], pitch[3], pitch[4], pitch[5], start, counts, n, err); \
+    break; \
+  }
+#define RUN_D(D) RUN(D, 16) RUN(D, 32) RUN(D, 64) RUN(D, 128)
+  switch (c->D * 1000 + blk) {
+    RUN_D(32) RUN_D(64) RUN_D(96) RUN_D(128)
+    default: return -1;
+  }
+#undef RUN_D
 #undef RUN
   return cudaGetLastError() == cudaSuccess ? 0 : -10;
 }
@@ -301,7 +316,7 @@ B200_API int b200_kv8_rope_append(const Kv8Cache* c, void* qkv, long long ld, in
 B200_API int b200_kv8_decode(const Kv8Cache* c, const int* lens, void* k_out, void* v_out, int L, int most, int* nan_first, int n, void* stream) {
   if (!kv8_cache_ok(c) || L <= 0 || most > L || most > c->cap || (!lens && L > c->cap)) return -1;
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return -2;
-  const long long vecs = static_cast<long long>(L) * c->Hkv * (c->D / 8);
+  const long long vecs = static_cast<long long>((L + 3) / 4) * c->Hkv * (c->D / 8);
   if (vecs > (1ll << 38)) return -3;
   launch_k(kv8_decode_kernel, dim3(static_cast<unsigned>((vecs + 255) / 256), 2, c->B), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), *c, lens,
            static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), L, most, c->Hkv * c->D, lens ? nan_first : nullptr, n);

@@ -67,13 +67,18 @@ struct LatentAttnParams {
   float cap_log2, cap_exp;      // cap in log2 units; exponent of e^(2 score / cap) per raw score, log2 units
   int keep;                     // keys of a sequence that stay visible beside the window
   float cap_poly[3], poly_max;  // capped log2 score = raw * polynomial(raw^2) for |raw| <= poly_max
+  // PARTS (and `group`): the key blocks of a tile are divided between `parts` CTAs, whose sums la_join_kernel puts together
+  int parts;
+  float4* part_o;               // [tile][head][part][vdim / 4][256 queries]: sums of weighted values
+  float2* part_ml;              // [tile][head][part][256 queries]: reference (-inf: nothing seen), sum of weights
 };
-enum AttnKind { LATENT = 0, BIAS = 1, CAPPED = 2, BOUNDED = 3, KEPT = 4, SMALL = 5 };
+enum AttnKind { LATENT = 0, BIAS = 1, CAPPED = 2, BOUNDED = 3, KEPT = 4, SMALL = 5, PARTS = 6 };
 __host__ __device__ constexpr bool la_bounded(int kind) { return kind == BOUNDED || kind == SMALL; }     // no running maximum
 __host__ __device__ constexpr bool la_keeps(int kind) { return kind == KEPT || kind == SMALL; }
 __host__ __device__ constexpr int la_softmax_warps(int kind) { return la_bounded(kind) ? 16 : 8; }
 __host__ __device__ constexpr int la_threads(int kind) { return 32 * (la_softmax_warps(kind) + 4); }
 // Columns in front of distance 0 and behind the last stored one (repeating the values there): a block's accesses need no clamps.
+constexpr int LA_MAX_PARTS = 4;
 constexpr int LA_BIAS_LEAD = 256, LA_BIAS_TAIL = 256;
 
 // The wait names the registers of the load: nothing that reads them moves in front of it.
@@ -150,7 +155,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQn, const __grid_consta
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int h = blockIdx.x, hk = KIND != LATENT ? h / p.group : h;
-  const int4 tile = p.tiles[blockIdx.y];
+  const int n_parts = KIND == PARTS ? p.parts : 1, tile_i = KIND == PARTS ? blockIdx.y / n_parts : blockIdx.y, part_i = blockIdx.y - tile_i * n_parts;
+  const int4 tile = p.tiles[tile_i];
   const int q0 = tile.x, nrows = tile.y, s0 = tile.z, kbase = tile.w;
   int kstart = max(kbase, s0 - p.window + 1);
   // key blocks [jb, je) of both tiles: nkb blocks of kept keys, the others counted from kstart
@@ -164,11 +170,25 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQn, const __grid_consta
       }
     }
   }
+  int blocks = INT_MAX;                     // PARTS: of this CTA
+  const size_t cell = (static_cast<size_t>(tile_i) * p.H + h) * n_parts + part_i;
+  if constexpr (KIND == PARTS) {
+    if (nrows <= 0) return;
+    // every part with blocks begins with a key that the tile's first query sees: no query of it is without one
+    const int all = (s0 + nrows - 1 - kbase) / BN + 1, seen = (s0 - kbase) / BN;
+    const int b0 = min(all * part_i / n_parts, seen), b1 = part_i + 1 == n_parts ? all : min(all * (part_i + 1) / n_parts, seen);
+    if (b0 >= b1) {
+      for (int r = threadIdx.x; r < nrows; r += la_threads(KIND)) p.part_ml[cell * 256 + r] = make_float2(-INFINITY, 0.f);
+      return;
+    }
+    kstart = kbase + b0 * BN;
+    blocks = b1 - b0;
+  }
   const bool keeps = la_keeps(KIND) && p.keep > 0;
   const int last_a = min(LA_BM, nrows) - 1, last_b = nrows - 1;
-  const int je0 = nkb + (s0 + last_a - kstart) / BN + 1;
-  const int jb1 = nrows > LA_BM && !keeps ? (max(kbase, s0 + LA_BM - p.window + 1) - kstart) / BN : 0;
-  const int je1 = nrows > LA_BM ? nkb + (s0 + last_b - kstart) / BN + 1 : 0;
+  const int je0 = min(nkb + (s0 + last_a - kstart) / BN + 1, blocks);
+  const int jb1 = nrows > LA_BM && !keeps && KIND != PARTS ? (max(kbase, s0 + LA_BM - p.window + 1) - kstart) / BN : 0;
+  const int je1 = nrows > LA_BM ? min(nkb + (s0 + last_b - kstart) / BN + 1, blocks) : 0;
   const int nmax = max(je0, je1);
   auto block_key = [&](int j) { return la_keeps(KIND) ? (j < nkb ? kbase + j * BN : kstart + (j - nkb) * BN) : kstart + j * BN; };   // first key of a block
 
@@ -523,7 +543,26 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQn, const __grid_consta
       const bool live = r < nrows;
       const size_t t = live ? static_cast<size_t>(q0) + r : 0;
       __nv_bfloat16* orow = p.out + t * p.ld_out + h * p.vdim;
-      if constexpr (KIND != LATENT) {
+      if constexpr (KIND == PARTS) {
+        if (live) p.part_ml[cell * 256 + r] = make_float2(m, l);
+        if (mbar_wait(&bars->o_final[x], 0, abort_flag, p.err, ERR_WAIT_ATTN)) {
+          tc_fence_after();
+          float4* to_part = p.part_o + cell * (p.vdim / 4) * 256 + r;
+#pragma unroll 1
+          for (int c = 0; c < p.vdim; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32(to + c, v);
+            tmem_ld_wait();
+            if (live) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                if (c + 4 * q < p.vdim)
+                  to_part[(c / 4 + q) * 256] = make_float4(__uint_as_float(v[4 * q]), __uint_as_float(v[4 * q + 1]), __uint_as_float(v[4 * q + 2]),
+                                                           __uint_as_float(v[4 * q + 3]));
+            }
+          }
+        }
+      } else if constexpr (KIND != LATENT) {
         float g = 1.f, den = l;
         if constexpr (KIND == BIAS) g = p.gate_mult / (1.f + __expf(-bf2f(p.gate[t * p.ld_gate + h])));
         if constexpr (KIND >= CAPPED)
@@ -604,6 +643,47 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQn, const __grid_consta
   }
 }
 
+// Puts the parts of a tile together: a CTA per 32 queries (lanes) of a tile and head, its warps take turns at eight channels.
+__global__ void __launch_bounds__(128)
+la_join_kernel(const LatentAttnParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int4 tile = p.tiles[blockIdx.x];
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, r = blockIdx.z * 32 + (threadIdx.x & 31);
+  if (r >= tile.y) return;
+  const size_t cell = (static_cast<size_t>(blockIdx.x) * p.H + h) * p.parts;
+  float f[LA_MAX_PARTS], l[LA_MAX_PARTS], top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < LA_MAX_PARTS; ++i) {
+    const float2 ml = i < p.parts ? p.part_ml[(cell + i) * 256 + r] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml.x);
+    f[i] = ml.x;
+    l[i] = ml.y;
+  }
+#pragma unroll
+  for (int i = 0; i < LA_MAX_PARTS; ++i) {
+    f[i] = f[i] == -INFINITY ? 0.f : ex2_approx(f[i] - top);
+    sum += f[i] > 0.f || l[i] != l[i] ? f[i] * l[i] : 0.f;      // a query whose scores are all NaN has no reference
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  __nv_bfloat16* out = p.out + (static_cast<size_t>(tile.x) + r) * p.ld_out + h * p.vdim;
+#pragma unroll 2
+  for (int c = 8 * warp; c < p.vdim; c += 32) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll
+    for (int i = 0; i < LA_MAX_PARTS; ++i) {
+      if (f[i] > 0.f) {                       // what a part without keys would hold was never written
+        const float4* o = p.part_o + ((cell + i) * (p.vdim / 4) + c / 4) * 256 + r;
+        const float4 y = o[0], z = o[256];
+        a.x = fmaf(y.x, f[i], a.x); a.y = fmaf(y.y, f[i], a.y); a.z = fmaf(y.z, f[i], a.z); a.w = fmaf(y.w, f[i], a.w);
+        b.x = fmaf(z.x, f[i], b.x); b.y = fmaf(z.y, f[i], b.y); b.z = fmaf(z.z, f[i], b.z); b.w = fmaf(z.w, f[i], b.w);
+      }
+    }
+    *reinterpret_cast<uint4*>(out + c) = make_uint4(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv), pack_bf16x2(b.x * inv, b.y * inv),
+                                                    pack_bf16x2(b.z * inv, b.w * inv));
+  }
+}
+
 typedef CUresult (*EncodeTiledFnL)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                    const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -655,12 +735,14 @@ static LatentAttnPlan latent_attn_plan(int dim, int rot, int vdim) {
 template <int BN, int SN, int SR, int KIND = LATENT>
 static int launch_latent_attn(const CUtensorMap* tm, const LatentAttnParams& p, const LatentAttnPlan& plan, int n_tiles, cudaStream_t st) {
   auto kern = latent_attn_kernel<BN, SN, SR, KIND>;
-  static int configured = 0;
-  if (configured < plan.smem) {
+  int dev = 0;
+  static int configured[64] = {};
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -10;
+  if (configured[dev] < plan.smem) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem) != cudaSuccess) return -10;
-    configured = plan.smem;
+    configured[dev] = plan.smem;
   }
-  kern<<<dim3(p.H, n_tiles), la_threads(KIND), plan.smem, st>>>(tm[0], tm[1], tm[2], tm[3], tm[4], p);
+  kern<<<dim3(p.H, n_tiles * (KIND == PARTS ? p.parts : 1)), la_threads(KIND), plan.smem, st>>>(tm[0], tm[1], tm[2], tm[3], tm[4], p);
   return cudaGetLastError() == cudaSuccess ? 0 : -11;
 }
 
@@ -804,4 +886,60 @@ B200_API int b200_capped_attention(const void* q, const void* k, const void* v, 
   if (small) return dispatch_grouped<SMALL>(tm, p, plan, n_tiles, st);
   if (keep > 0) return dispatch_grouped<KEPT>(tm, p, plan, n_tiles, st);
   return bounded ? dispatch_grouped<BOUNDED>(tm, p, plan, n_tiles, st) : dispatch_grouped<CAPPED>(tm, p, plan, n_tiles, st);
+}
+
+// How many CTAs share the keys of a tile (1: none do): the fewest that bring the time to its minimum, counted in key blocks of the busiest SM.
+// A CTA costs about two blocks beside its own, and joining a part of a wave of tiles one more.  (1500 queries, 32 heads of 128, 7777 keys: 192
+// CTAs are two rounds of the machine for 1.3 rounds of work; 3 parts take XX us, none YY.)
+B200_API int b200_attention_parts(int n_tiles, int H, int keys) {
+  int dev = 0, sms = 0;
+  if (n_tiles <= 0 || H <= 0 || keys <= 0 || cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+    return 1;
+  const long long ctas = static_cast<long long>(n_tiles) * H;
+  const int blocks = (keys + 127) / 128;
+  if (ctas > 4ll * sms) return 1;
+  int best = 1;
+  double least = 0;
+  for (int parts = 1; parts <= LA_MAX_PARTS; ++parts) {
+    const double rounds = static_cast<double>((ctas * parts + sms - 1) / sms);
+    const double cost = rounds * ((blocks + parts - 1) / parts + 2) + (parts > 1 ? 2 + parts * static_cast<double>(ctas) / sms : 0.0);
+    if (parts == 1 || cost < 0.95 * least) { best = parts; least = cost; }
+  }
+  return best;
+}
+
+// As above without caps, sinks, windows and kept keys; tiles with the keys of their sequence from the first on.  part_o: float4 [n_tiles * H * parts *
+// vdim / 4 * 256], part_ml: float2 [n_tiles * H * parts * 256].
+B200_API int b200_parted_attention(const void* q, const void* k, const void* v, void* out, const int* tiles, void* part_o, void* part_ml, int parts,
+                                   int n_tiles, int T, int K, int H, int G, int dim, int vdim, int ld_q, int ld_kv, int ld_out, float scale,
+                                   void* stream, int* err) {
+  const LatentAttnPlan plan = latent_attn_plan(dim, 0, vdim);
+  if (!plan.bn || n_tiles <= 0 || parts < 1 || parts > LA_MAX_PARTS || static_cast<long long>(n_tiles) * parts > 65535 || H <= 0 || H > 65535 || G <= 0 ||
+      H % G || T <= 0 || K <= 0 || !(scale > 0.f)) return -1;
+  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(part_o)) & 15) || (reinterpret_cast<uintptr_t>(part_ml) & 7) || (ld_out & 7)) return -2;
+  CUtensorMap tm[5];
+  int rc = make_tmap_rows(&tm[0], q, dim, H, T, dim, ld_q, LA_BM);
+  if (!rc) rc = make_tmap_rows(&tm[2], k, dim, G, K, dim, ld_kv, plan.bn);
+  if (!rc) rc = make_tmap_rows(&tm[4], v, vdim, G, K, vdim, ld_kv, plan.bn);
+  if (rc) return rc;
+  tm[1] = tm[0];
+  tm[3] = tm[2];
+  LatentAttnParams p = {};
+  p.H = H; p.dim = dim; p.rot = 0; p.vdim = vdim; p.window = 1 << 30;
+  p.pn = (dim + 63) / 64; p.pr = 0; p.pv = (vdim + 63) / 64;
+  p.kst = plan.kst; p.vst = plan.vst;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.tiles = reinterpret_cast<const int4*>(tiles);
+  p.out = reinterpret_cast<__nv_bfloat16*>(out); p.ld_out = ld_out;
+  p.err = err;
+  p.group = H / G;
+  p.parts = parts;
+  p.part_o = static_cast<float4*>(part_o);
+  p.part_ml = static_cast<float2*>(part_ml);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  rc = dispatch_grouped<PARTS>(tm, p, plan, n_tiles, st);
+  if (rc) return rc;
+  launch_k(la_join_kernel, dim3(n_tiles, H, 8), dim3(128), 0, st, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -12;
 }

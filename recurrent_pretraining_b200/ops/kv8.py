@@ -58,7 +58,8 @@ def _k():
             nan=K._sig("b200_kv8_nan", [vp] * 3 + [i] * 6 + [vp]),
             plan=K._sig("b200_kv8_attention_plan", [i] * 5 + [C.POINTER(i)]),
             attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn)] + [vp] * 5),
-            long_ok=K._sig("b200_capped_attention_supported", [i, i]),
+            parts=K._sig("b200_attention_parts", [i] * 3),
+            parted=K._sig("b200_parted_attention", [vp] * 7 + [i] * 11 + [C.c_float, vp, vp]),
             long=K._sig("b200_capped_attention", [vp] * 6 + [i] * 12 + [C.c_float] * 3 + [vp, vp]),
         )
     return _fns
@@ -334,8 +335,15 @@ def _long(q, cache, lens, scale, most) -> torch.Tensor:
         nans = torch.empty(B, W, dtype=torch.int32, device=cache.device)
         K._check(f.tiles(lens.data_ptr(), tiles.data_ptr(), out.data_ptr(), B, n, most, L, H * D, nans.data_ptr(), W, st), "kv8_tiles")
         K._check(f.decode(C.byref(cache._c), lens.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), L, most, nans.data_ptr(), n, st), "kv8_decode")
-        K._check(f.long(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), 0, B * per, B * n, B * L, H, Hkv, D, D,
-                        H * D, W, H * D, 2 ** 30, 0, scale, 0.0, 0.0, st, K.err_word(cache.device).data_ptr()), "capped_attention")
+        parts = f.parts(B * per, H, most)
+        if parts > 1:
+            cells = B * per * H * parts * 256
+            sums, refs = (torch.empty(cells * w, dtype=F32, device=cache.device) for w in (D, 2))
+            K._check(f.parted(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), sums.data_ptr(), refs.data_ptr(), parts,
+                              B * per, B * n, B * L, H, Hkv, D, D, H * D, W, H * D, scale, st, K.err_word(cache.device).data_ptr()), "parted_attention")
+        else:
+            K._check(f.long(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), 0, B * per, B * n, B * L, H, Hkv, D, D,
+                            H * D, W, H * D, 2 ** 30, 0, scale, 0.0, 0.0, st, K.err_word(cache.device).data_ptr()), "capped_attention")
         K._check(f.nan(nans.data_ptr(), lens.data_ptr(), out.data_ptr(), B, n, H // Hkv, Hkv, D, most, st), "kv8_nan")
         return out
 

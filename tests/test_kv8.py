@@ -278,6 +278,9 @@ CASES = [  # B, n, H, Hkv, D, block, cap, lens
     (3, 100, 6, 6, 96, 16, 304, [300, 99, 0]),
     (1, 300, 4, 2, 128, 32, 608, [601]),
     (2, 270, 2, 1, 32, 32, 320, [320, 13]),
+    (2, 257, 4, 1, 128, 128, 1664, [1650, 258]),       # a tile of one query
+    (1, 160, 2, 2, 96, 16, 1008, [1000]),
+    (3, 400, 20, 10, 64, 32, 480, [433, 401, 127]),
 ]
 
 
@@ -367,6 +370,7 @@ def test_long_attention_nan_reaches_only_those_who_see_it(device):
     q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(device)
     lens = i32([400, 75], device)
     clean = kv8.attention(q, cache, lens)
+    q[0, 3, 1] = float("nan")
     v, k = cache.v.view(torch.uint8), cache.k.view(torch.uint8)
     v[0, 0, 390, 5] = v[0, 0, 395, 5] = 0x7F                # seen by the last ten tokens
     v[0, 0, 20, 6] = 0xFF                                   # by all
@@ -374,6 +378,7 @@ def test_long_attention_nan_reaches_only_those_who_see_it(device):
     v[1, 1, 74, 0] = v[1, 1, 5, 1] = 0x7F                   # by the last one; by all
     out = kv8.attention(q, cache, lens)
     nan = torch.zeros(B, n, H, D, dtype=torch.bool)
+    nan[0, 3, 1] = True
     nan[0, 60:, :2, 5] = nan[0, :, :2, 6] = nan[0, 69, 2:] = nan[1, 69, 2:, 0] = nan[1, :, 2:, 1] = True
     assert torch.equal(out.isnan().cpu(), nan)
     assert torch.equal(out[~out.isnan()], clean[~out.isnan()])
