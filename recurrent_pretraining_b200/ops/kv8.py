@@ -54,14 +54,12 @@ def _k():
             append=K._sig("b200_kv8_append", [C.POINTER(_Cache), vp, vp, C.POINTER(ll), vp, vp, i, vp, vp]),
             rope=K._sig("b200_kv8_rope_append", [C.POINTER(_Cache), vp, ll, i, i, vp, vp, vp, vp, vp, i, vp, vp]),
             decode=K._sig("b200_kv8_decode", [C.POINTER(_Cache), vp, vp, vp, i, i, vp, i, vp]),
-            tiles=K._sig("b200_kv8_tiles", [vp, vp, vp, i, i, i, i, ll, vp, i, vp]),
-            nan=K._sig("b200_kv8_nan", [vp] * 3 + [i] * 6 + [vp]),
             plan=K._sig("b200_kv8_attention_plan", [i] * 5 + [C.POINTER(i)]),
             attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn)] + [vp] * 5),
-            parts=K._sig("b200_attention_parts", [i] * 3),
-            parted=K._sig("b200_parted_attention", [vp] * 7 + [i] * 11 + [C.c_float, vp, vp]),
-            long=K._sig("b200_capped_attention", [vp] * 6 + [i] * 12 + [C.c_float] * 3 + [vp, vp]),
+            scratch=K._sig("b200_kv8_prompt_scratch", [i] * 6),
+            prompt=K._sig("b200_kv8_prompt", [C.POINTER(_Cache)] + [vp] * 4 + [i] * 3 + [C.c_float, vp, vp]),
         )
+        _fns.scratch.restype = C.c_longlong
     return _fns
 
 
@@ -276,7 +274,7 @@ def _attention_call(cache, q, lens, scale, max_len):
         return lambda cache, q, lens: ref.kv8_attention(q, cache, lens, scale, most)
     group = H // cache.kv_heads
     if n * group > STREAM_ROWS and scale > 0:
-        return lambda cache, q, lens: _long(q, cache, lens, scale, most)
+        return _prompt_call(cache, q, scale, most)
     ok = _aligned(q)
     f, c, device = _k(), cache._c, cache.device
     plan = (C.c_int * 4)()
@@ -315,36 +313,25 @@ def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optio
     return cache._call((_kind(q), _kind(lens), scale, max_len), _attention_call, q, lens, scale, max_len)(cache, q, lens)
 
 
-def _long(q, cache, lens, scale, most) -> torch.Tensor:
+def _prompt_call(cache, q, scale, most):
     """Many query rows per key: the codes become bf16 rows once (exactly), and the prompt attention on the tensor cores reads those."""
-    f = _k()
     B, n, H, D = q.shape
-    Hkv, W = cache.kv_heads, cache.kv_heads * D
-    L = (most + 127) // 128 * 128
-    if not q.is_contiguous() or q.data_ptr() & 15:
-        q = _copy(q)
-    per = (n + 255) // 256
-    if B * per > 65535 or B * max(L, n) >= 2 ** 31:
+    f, device, c, empty_like = _k(), cache.device, C.byref(cache._c), torch.empty_like
+    nbytes = _guarded(device, lambda: f.scratch(B, cache.kv_heads, H, D, n, most))
+    if not nbytes:
         raise ValueError(f"{B} sequences of {n} tokens and {most} keys are too many for one call")
+    like, mem_like = (torch.empty(1, dtype=t, device=device).expand(s) for t, s in ((BF16, q.shape), (torch.uint8, (nbytes,))))
+    err, contiguous, layout = f.K.err_word(device).data_ptr(), q.is_contiguous(), torch.contiguous_format
 
-    def run():
-        K, st = f.K, f.K._stream()
-        out = torch.empty(B, n, H, D, dtype=BF16, device=cache.device)
-        kv = torch.empty(2, B * L, W, dtype=BF16, device=cache.device)
-        tiles = torch.empty(B * per, 4, dtype=torch.int32, device=cache.device)
-        nans = torch.empty(B, W, dtype=torch.int32, device=cache.device)
-        K._check(f.tiles(lens.data_ptr(), tiles.data_ptr(), out.data_ptr(), B, n, most, L, H * D, nans.data_ptr(), W, st), "kv8_tiles")
-        K._check(f.decode(C.byref(cache._c), lens.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), L, most, nans.data_ptr(), n, st), "kv8_decode")
-        parts = f.parts(B * per, H, most)
-        if parts > 1:
-            cells = B * per * H * parts * 256
-            sums, refs = (torch.empty(cells * w, dtype=F32, device=cache.device) for w in (D, 2))
-            K._check(f.parted(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), sums.data_ptr(), refs.data_ptr(), parts,
-                              B * per, B * n, B * L, H, Hkv, D, D, H * D, W, H * D, scale, st, K.err_word(cache.device).data_ptr()), "parted_attention")
+    def run(cache, q, lens):            # holds no reference to the cache, which holds this
+        if not contiguous or q.data_ptr() & 15:
+            q = _copy(q)
+        out, mem = empty_like(like, memory_format=layout), empty_like(mem_like, memory_format=layout)
+        if device.index == _device():
+            f.check(f.prompt(c, q.data_ptr(), lens.data_ptr(), out.data_ptr(), mem.data_ptr(), H, n, most, scale, err, f.stream()), "kv8_prompt")
         else:
-            K._check(f.long(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), tiles.data_ptr(), 0, B * per, B * n, B * L, H, Hkv, D, D,
-                            H * D, W, H * D, 2 ** 30, 0, scale, 0.0, 0.0, st, K.err_word(cache.device).data_ptr()), "capped_attention")
-        K._check(f.nan(nans.data_ptr(), lens.data_ptr(), out.data_ptr(), B, n, H // Hkv, Hkv, D, most, st), "kv8_nan")
+            with torch.cuda.device(device):
+                f.check(f.prompt(c, q.data_ptr(), lens.data_ptr(), out.data_ptr(), mem.data_ptr(), H, n, most, scale, err, f.stream()), "kv8_prompt")
         return out
 
-    return _guarded(cache.device, run)
+    return run
