@@ -27,6 +27,7 @@ import torch
 from ..models.sampling import SamplingOptions
 from ..ops import cuda as K
 from ..ops import kv8
+from ..ops.reference import KV8_EMIN
 from ..ops.sampling import sample_tokens
 from .base import BF16, PDL, SKINNY_ROWS, GraphRunner, skinny_linear
 
@@ -89,7 +90,7 @@ class StaticRecurrentKV8Cache(StaticRecurrentKVCache):
         blocks = (max_len + block - 1) // block
         self.k, self.v = (torch.zeros(n_slots, batch, n_kv, blocks * block, head_dim, dtype=torch.uint8, device=device).view(kv8.E4M3)
                           for _ in range(2))
-        self.k_exp, self.v_exp = (torch.zeros(n_slots, batch, n_kv, blocks, dtype=torch.int8, device=device) for _ in range(2))
+        self.k_exp, self.v_exp = (torch.full((n_slots, batch, n_kv, blocks), KV8_EMIN, dtype=torch.int8, device=device) for _ in range(2))
         self.layers = [kv8.KV8Cache(self.k[s], self.v[s], self.k_exp[s], self.v_exp[s]) for s in range(n_slots)]
         self._seen_tokens = 0
 
@@ -153,6 +154,8 @@ class DecodeEngine(GraphRunner):
         self.init_buf = torch.zeros_like(self.state)                            # fresh random state per token
         self.tok_out = torch.zeros(max_batch, dtype=torch.int64, device=d)
         self.uniform = torch.zeros(max_batch, dtype=torch.float32, device=d)   # numbers that the next token is drawn from
+        self.sampling = {k: torch.zeros(max_batch, dtype=torch.int32 if k == "top_k" else torch.float32, device=d)
+                         for k in ("temperature", "top_k", "top_p", "min_p")}
         self.next_state = torch.zeros_like(self.state)
         self._seed = 1
         self.logits = torch.zeros(max_batch, self.V, dtype=torch.float32, device=d)
@@ -284,18 +287,22 @@ class DecodeEngine(GraphRunner):
             self.init_buf.copy_(K.trunc_normal(self.init_buf.shape, std, self._seed, BF16, self.dev))
 
     # -- public API ---------------------------------------------------------------------------------------
-    @staticmethod
-    def _settings(sampling: SamplingOptions | None) -> dict | None:
-        """Arguments of ``sample_tokens``; None: greedy."""
+    def _settings(self, sampling: SamplingOptions | None) -> bool:
+        """Whether tokens are sampled; their settings go where a captured step reads them (one graph serves all settings)."""
         if sampling is None or sampling.greedy:
-            return None
+            return False
         if sampling.repetition_penalty not in (None, 1.0):
             raise ValueError("the recurrent decode engine has no repetition penalty")
-        return dict(temperature=float(sampling.temperature or 1.0), top_k=int(sampling.top_k or 0), top_p=float(sampling.top_p or 1.0),
-                    min_p=float(sampling.min_p or 0.0))
+        given = dict(temperature=float(sampling.temperature or 1.0), top_k=int(sampling.top_k or 0), top_p=float(sampling.top_p or 1.0),
+                     min_p=float(sampling.min_p or 0.0))
+        if not (given["temperature"] > 0 and 0 <= given["top_k"] < 2 ** 31 and 0 <= given["top_p"] <= 1 and 0 <= given["min_p"] <= 1):
+            raise ValueError(f"sampling needs temperature > 0, top_k >= 0, top_p and min_p in 0 .. 1: got {given}")
+        for name, x in given.items():
+            self.sampling[name].fill_(x)
+        return True
 
-    def _pick(self, logits, settings: dict | None):
-        return logits.argmax(-1) if settings is None else sample_tokens(logits, self.uniform[:logits.shape[0]], **settings)
+    def _pick(self, logits, sampled: bool):
+        return sample_tokens(logits, self.uniform, **self.sampling) if sampled else logits.argmax(-1)
 
     @torch.no_grad()
     def prefill(self, input_ids: torch.Tensor, num_steps: int | None = None, init_scale: float = 1.0,
@@ -313,7 +320,7 @@ class DecodeEngine(GraphRunner):
         self.lens.fill_(P + 1)
         return self.tok.clone()
 
-    def _token_fixed(self, r: int, continuous: bool, settings: dict | None = None):
+    def _token_fixed(self, r: int, continuous: bool, sampled: bool = False):
         """Graph body: token ``tok`` at position ``pos`` -> ``tok_out`` / ``state_out`` (inputs are not modified)."""
         e = self._embed()
         s = self.state if continuous else self.init_buf
@@ -321,7 +328,7 @@ class DecodeEngine(GraphRunner):
             s = self._recurrence(s, e, step)
         logits = self._head(s)
         self.state_out.copy_(s)
-        self.tok_out.copy_(self._pick(logits, settings))
+        self.tok_out.copy_(self._pick(logits, sampled))
         return self.tok_out
 
     @torch.no_grad()
@@ -335,10 +342,10 @@ class DecodeEngine(GraphRunner):
         r = num_steps or self.r
         B, P = input_ids.shape
         assert P + max_new_tokens <= self.Lmax
-        settings = self._settings(sampling)
-        if settings is not None and criterion is not None:
+        sampled = self._settings(sampling)
+        if sampled and criterion is not None:
             raise ValueError("sampling goes with a fixed number of recurrences")
-        if settings is not None:
+        if sampled:
             self.uniform.uniform_(generator=generator)
         first = self.prefill(input_ids, r, init_scale, sampling)
         out = [first]
@@ -347,10 +354,10 @@ class DecodeEngine(GraphRunner):
             for _ in range(max_new_tokens - 1):
                 if not continuous_compute:
                     self._fresh_state(init_scale)
-                if settings is not None:
+                if sampled:
                     self.uniform.uniform_(generator=generator)
-                key = ("fixed", r, continuous_compute) + (() if settings is None else tuple(settings.values()))
-                self._run(key, lambda: self._token_fixed(r, continuous_compute, settings))
+                key = ("fixed", r, continuous_compute) + (("sampled",) if sampled else ())
+                self._run(key, lambda: self._token_fixed(r, continuous_compute, sampled))
                 self.tok.copy_(self.tok_out)
                 self.state.copy_(self.state_out)
                 self.pos.add_(1)

@@ -99,6 +99,13 @@ def test_sampled_tokens(model, kv_dtype):
     options = dict(temperature=1.5, top_k=200, top_p=0.95)
     eng.uniform[:2] = numbers
     assert torch.equal(eng._pick(logits, eng._settings(SamplingOptions(do_sample=True, **options))), sample_tokens(logits, numbers, **options))
+    graphs = len(eng._graphs)
+    for t in (0.3, 0.31, 0.32):
+        run(9, temperature=t, top_p=0.5 + t)
+    assert len(eng._graphs) == graphs                        # requests' settings need no graphs of their own
+    for bad in (dict(temperature=-1.0), dict(top_k=-2), dict(top_p=1.5), dict(min_p=-0.1)):
+        with pytest.raises(ValueError):
+            run(9, **bad)
     assert torch.equal(eng.generate(ids, 10, init_scale=0.0, sampling=SamplingOptions(temperature=3.0))[0], greedy)      # do_sample is off
     with pytest.raises(ValueError):
         eng.generate(ids, 4, criterion="kl", sampling=SamplingOptions(do_sample=True))
