@@ -10,7 +10,7 @@ again forgets what lies behind it in the block.  Infinities are stored as the bl
 
 Sequences are described by int32 tensors on the cache's device and never read by the host: positions outside the cache are left out by
 the kernels (nothing is written) and recorded in the device status word (``cuda.check_device_status``), lengths are cut to the capacity.
-Calls run on the current stream and allocate through PyTorch's allocator."""
+Calls run on the current stream and allocate through PyTorch's allocator.  They belong to decoding: none has a gradient."""
 from __future__ import annotations
 
 import ctypes as C
@@ -109,6 +109,8 @@ class KV8Cache:
             raise ValueError("a cache has at least one sequence, head and position")
         if k.stride()[2:] != (self.dim, 1) or v.stride() != k.stride() or ke.stride(2) != 1 or ve.stride() != ke.stride():
             raise ValueError("a head's positions are contiguous, and keys and values laid out alike")
+        if not (_apart(k, self.capacity * self.dim) and _apart(ke, blocks)):
+            raise ValueError("heads do not overlap")
         if k.is_cuda and ((k.data_ptr() | v.data_ptr() | k.stride(0) | k.stride(1)) & 15):
             raise ValueError("heads start on 16-byte boundaries")
         self.device = k.device
@@ -142,6 +144,16 @@ class KV8Cache:
                 self._calls.clear()
             call = self._calls[key] = make(self, *args)
         return call
+
+
+def _apart(t: torch.Tensor, extent: int) -> bool:
+    """Whether the heads [B, kv_heads] of ``extent`` elements each lie in places of their own."""
+    for stride, n in sorted(zip(t.stride()[:2], t.shape[:2])):
+        if n > 1:
+            if stride < extent:
+                return False
+            extent = stride * (n - 1) + extent
+    return True
 
 
 def _index(t: torch.Tensor, cache: KV8Cache, what: str) -> None:
@@ -220,8 +232,8 @@ def _rope_call(cache, qkv, cos, sin, pos, heads, bias, clear):
             raise ValueError(f"{what} is a contiguous fp32 table [>= {cache.capacity}, {D // 2}] on the cache's device")
     if bias is not None and (bias.dtype != F32 or bias.numel() != (heads + Hkv) * D or not bias.is_contiguous() or bias.device != cache.device):
         raise ValueError(f"bias is a contiguous fp32 tensor of {(heads + Hkv) * D} values on the cache's device")
-    if clear and qkv.dtype != F32:
-        raise ValueError("only an fp32 accumulator is handed back zeroed")
+    if clear and (qkv.dtype != F32 or (B > 1 and qkv.stride(0) < W)):
+        raise ValueError("only an fp32 accumulator whose rows do not overlap is handed back zeroed")
     _index(pos, cache, "pos")
     ld = 0 if B == 1 else qkv.stride(0)
     err = _k().K.err_word(cache.device).data_ptr() if cache.k.is_cuda else 0

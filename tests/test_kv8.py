@@ -427,12 +427,18 @@ def test_refusals():
         lambda: kv8.attention(q.float(), cache, p), lambda: kv8.attention(q[:, :, :3], cache, p), lambda: kv8.attention(q[:1], cache, p),
         lambda: kv8.attention(q, cache, p.long()), lambda: kv8.attention(q, cache, p, max_len=0), lambda: kv8.attention(q, cache, p, max_len=65),
         lambda: kv8.attention(q[..., :16], cache, p),
+        lambda: KV8Cache(*(t[:1].expand(2, *t.shape[1:]) for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_exp, cache.v_exp))),
+        lambda: KV8Cache(*(t[:1].expand(2, *t.shape[1:]) for t in (cache.k, cache.v, cache.k_exp, cache.v_exp))),      # two sequences in one place
+        lambda: KV8Cache(cache.k, cache.v, *(t[:, :1].expand(2, 2, 2) for t in (cache.k_exp, cache.v_exp))),
+        lambda: kv8.rope_append(cache, qkv[:1].expand(2, -1), cos, sin, p, 4, clear=True),
+        lambda: kv8.rope_append(cache, torch.zeros(300).as_strided((2, 256), (32, 1)), cos, sin, p, 4, clear=True),
     ]
     for i, f in enumerate(bad):
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"call {i} was taken")
     kv8.append(cache, k[:, :0], k[:, :0], p)      # nothing to write
+    KV8Cache(*(t.transpose(0, 1) for t in (cache.k, cache.v, cache.k_exp, cache.v_exp)))       # heads in any order
 
 
 # ------------------------------------------------------------------------------------------
