@@ -23,7 +23,15 @@ from . import reference as ref
 
 BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
 BLOCKS = (16, 32, 64, 128)
-STREAM_ROWS = 64        # query tokens x heads per key head up to which the cache is streamed as it is
+
+
+def streams(n: int, dim: int) -> bool:
+    """Whether n query tokens per sequence are answered by streaming the codes, 32 rows (tokens x heads of a key head) at a time, and not from
+    bf16 rows by the prompt attention, whose tiles are filled by the tokens of one head.  Microseconds of both ways at 8 sequences of 4096 keys
+    and 8 key heads: dim 64, 4 heads per key head: 64 tokens 95 / 124, 128 tokens 176 / 126; dim 128, 1 head: 64 tokens 64 / 70, 128 tokens
+    99 / 72; 16 heads: 32 tokens 281 / 446, 64 tokens 537 / 447.  They are equal at about 105 (94), 95 (75), 80 (64) and 62 (52) tokens
+    for dims of 32, 64, 96 and 128 with 4 (16) heads per key head."""
+    return n <= 112 - dim // 2
 
 
 class _Cache(C.Structure):
@@ -285,7 +293,7 @@ def _attention_call(cache, q, lens, scale, max_len):
     if not cache.k.is_cuda:
         return lambda cache, q, lens: ref.kv8_attention(q, cache, lens, scale, most)
     group = H // cache.kv_heads
-    if n * group > STREAM_ROWS and scale > 0:
+    if not streams(n, D) and scale > 0:
         return _prompt_call(cache, q, scale, most)
     ok = _aligned(q)
     f, c, device = _k(), cache._c, cache.device

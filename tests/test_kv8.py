@@ -274,7 +274,11 @@ CASES = [  # B, n, H, Hkv, D, block, cap, lens
     (2, 9, 6, 2, 128, 16, 96, [96, 8]),                # 27 rows
     (2, 11, 12, 3, 96, 16, 560, [559, 10]),            # 44 rows: two row tiles
     (1, 64, 2, 2, 96, 64, 640, [631]),                 # 64 rows
-    (2, 33, 4, 2, 64, 32, 352, [345, 33]),             # 66 rows: the prompt kernel
+    (2, 33, 4, 2, 64, 32, 352, [345, 33]),             # 66 rows
+    (2, 9, 28, 2, 96, 32, 640, [640, 5]),              # 126 rows, tiles of 32 that begin inside a token
+    (1, 48, 6, 2, 128, 32, 1280, [1270]),
+    (1, 49, 6, 2, 128, 32, 1280, [1270]),              # from here on the prompt kernel
+    (2, 65, 4, 2, 96, 16, 352, [345, 66]),
     (3, 100, 6, 6, 96, 16, 304, [300, 99, 0]),
     (1, 300, 4, 2, 128, 32, 608, [601]),
     (2, 270, 2, 1, 32, 32, 320, [320, 13]),
@@ -297,7 +301,7 @@ def test_attention(device, B, n, H, Hkv, D, block, cap, lens):
     out = kv8.attention(q.to(device), cache, i32(lens, device)).double().cpu()
     k, v = (torch.nan_to_num(values(cache, w)) for w in "kv")
     want, mag, big = attend(q.double(), k, v, lens, D ** -0.5)
-    tol = tolerance(want, mag, big, D, BF16_HALF if n * (H // Hkv) > kv8.STREAM_ROWS else F16_HALF)
+    tol = tolerance(want, mag, big, D, F16_HALF if kv8.streams(n, D) else BF16_HALF)
     bad = (out - want).abs() > tol
     assert not bad.any(), ((out - want).abs() / tol).max()
 
@@ -365,7 +369,8 @@ def test_attention_nan_reaches_only_those_who_see_it(device):
 
 @pytest.mark.parametrize("device", DEVICES)
 def test_long_attention_nan_reaches_only_those_who_see_it(device):
-    B, n, H, Hkv, D, cap = 2, 70, 4, 2, 64, 416
+    B, n, H, Hkv, D, cap = 2, 70, 4, 2, 128, 416
+    assert not kv8.streams(n, D)
     cache = filled(B, Hkv, cap, D, 32, device)
     q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(device)
     lens = i32([400, 75], device)
