@@ -12,9 +12,10 @@
 // and divided further by the bits of their keys until few are left, which are ranked against each other.  Should they be too many to be
 // collected (equal logits), the whole slices are divided again, down to a single value whose ties are counted in index order.
 //
-// A row is bound by the latency of its stages: 17.5 us for 65536 fp32 logits with top-k 50 and top-p 0.9 (16 CTAs; read 1.6, maximum 0.8,
-// histogram 3, its exchange 3, candidates 2, ranking 2.5, kept list and its sums 2, the token 2), where 8 CTAs take 24 and the bytes 0.04.  A batch
-// of 64 such rows (4 CTAs each, two per SM) takes 41.5 us: it is bound by the instructions of the pass that forms the weights and the histogram.
+// A row is bound by the latency of its stages: 17.5 us for 65536 fp32 logits with top-p 0.95 on 16 CTAs (read 1.4, maximum 1.4, histogram 2.6, its
+// exchange and border 4.4, candidates 2, ranking 2.5, kept list 1.5, token 1.7), where the bytes would take 0.04.  A batch of 64 such rows with settings of
+// their own (4 CTAs each, two per SM) takes 41.5 us: 14 of them are the histogram pass, bound by the instructions that form the weights (atomics 3,
+// the table 1, both measured by leaving them out).
 #include <cooperative_groups.h>
 
 #include <utility>
@@ -451,7 +452,7 @@ sample_kernel(const SampleParams p) {
         r->xa[phase][rank] = static_cast<uint32_t>(a2);
         r->xb[phase][rank] = static_cast<uint32_t>(z2);
       }
-      clear();                                      // all have read and are done with the lists of this round
+      clear();                                      // all have read and are done with the present lists
       cluster.sync();
       kmin = 0xFFFFFFFFu;
       kmax = 0;
