@@ -10,7 +10,7 @@
 // them is encoded again by the CTA (or lane group) that writes them.  Writing the same tokens to the same place again
 // changes nothing: exponents only grow.  Nothing behind the new tokens is touched.
 //
-// Appending is bound by memory: 4 x 1024 tokens of 55 heads of 96 take 22.5 us, 5.8 TB/s of reads and writes mixed (28.1 with the magnitudes
+// Appending is bound by memory: 4 x 1024 tokens of 55 heads of 96 take 22.0 us, 5.9 TB/s of reads and writes mixed (28.1 with the magnitudes
 // compared as fp32 numbers: there were more instructions than the memory left time for).  A step's tokens (64 sequences, 48
 // heads of 128) take 2.6 us, about an empty launch.
 #include "kv8.cuh"
@@ -24,21 +24,22 @@ struct Kv8Cache {
   int B, Hkv, cap, D, log2_block;
 };
 
-// Values of a block up to which a warp takes it (4 x 1024 tokens of 55 heads of 96 in blocks of 32: 22.5 us with 128 threads to a block, 30.3 with a
-// warp).
-constexpr int KV8_WARP_VALUES = 1024;
+// Threads for a block of so many values, 24 to 96 values each.  4 x 1024 tokens of 5280 channels, 20 us of copying: 20.1 to 22.3 us with every block and
+// dim but 16 x 32 (25.1).  2048 values take 25.5 with 128 threads, 23.7 with 64, 21.8 with a warp; 16384 take 26.3 with 128 threads, 20.7 with 256.
+__host__ __device__ constexpr int kv8_group(int values) { return values <= 2048 ? 32 : values <= 12288 ? 128 : 256; }
+__host__ __device__ constexpr int kv8_threads(int G) { return G > 32 ? G : 128; }
 
 // grid (2 x most touched blocks / (128 / G), Hkv, B), 128 threads, G of them (a warp or the CTA) per block of BLK tokens.  The block's new tokens
 // stay in registers (NV vectors of eight values per thread) between the maximum and the encoding: one pass over the input.  D and BLK
 // are known to the compiler: a division per vector would take longer than the vector.
 template <int D, int BLK, int G>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kv8_threads(G))
 kv8_append_kernel(const Kv8Cache c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v, long long k_sb,
                   long long k_sn, long long k_sh, long long v_sb, long long v_sn, long long v_sh, const int* __restrict__ start_,
                   const int* __restrict__ counts, int n, int* err) {
   pdl_trigger();
   pdl_wait();
-  const int unit = blockIdx.x * (128 / G) + threadIdx.x / G, which = unit & 1, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x % G;
+  const int unit = blockIdx.x * (kv8_threads(G) / G) + threadIdx.x / G, which = unit & 1, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x % G;
   const int start = start_[b], cnt = counts ? counts[b] : n;
   if (start < 0 || cnt < 0 || cnt > n || start > c.cap - cnt) {     // the sequence does not fit: nothing of it is written
     if (tid == 0 && err) atomicCAS(err, 0, ERR_BAD_INDEX);
@@ -62,15 +63,15 @@ kv8_append_kernel(const Kv8Cache c, const __nv_bfloat16* __restrict__ k, const _
   }
   const bool fresh = lo == p0;
   const int old = fresh ? KV8_EMIN : *ep;
-  // magnitudes are compared as the 16-bit integers that they are; infinities and NaN, the largest of those, have to be looked at one by one
-  uint32_t top = 0;
+  // magnitudes are compared in pairs of bf16; where there is an infinity or NaN, which do not count, one by one
+  __nv_bfloat162 top = __float2bfloat162_rn(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
+    for (int j = 0; j < 4; ++j) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])));
   }
-  float amax = __uint_as_float(max(top << 16, top & 0xFFFF0000u));
+  float amax = __bfloat162float(__hmax_nan(__low2bfloat16(top), __high2bfloat16(top)));
   if (!(amax < INFINITY)) {
     amax = 0.f;
 #pragma unroll
@@ -85,10 +86,11 @@ kv8_append_kernel(const Kv8Cache c, const __nv_bfloat16* __restrict__ k, const _
   }
   amax = warp_max(amax);                                            // every thread has read the old exponent, too
   if constexpr (G > 32) {
-    __shared__ float red[4];
+    __shared__ float red[G / 32];
     if ((tid & 31) == 0) red[tid >> 5] = amax;
     __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int i = 0; i < G / 32; ++i) amax = fmaxf(amax, red[i]);
   }
   const int e = max(kv8_exponent(amax), old);
   const float inv = pow2i(-e);
@@ -295,8 +297,8 @@ B200_API int b200_kv8_append(const Kv8Cache* c, const void* k, const void* v, co
   const __nv_bfloat16 *kb = static_cast<const __nv_bfloat16*>(k), *vb = static_cast<const __nv_bfloat16*>(v);
 #define RUN(D, BLK) \
   case D * 1000 + BLK: { \
-    constexpr int G = BLK * D <= KV8_WARP_VALUES ? 32 : 128; \
-    launch_k(kv8_append_kernel<D, BLK, G>, dim3(static_cast<unsigned>((2 * touched + 128 / G - 1) / (128 / G)), c->Hkv, c->B), dim3(128), 0, st, *c, kb, vb, \
+    constexpr int G = kv8_group(BLK * D), per = kv8_threads(G) / G; \
+    launch_k(kv8_append_kernel<D, BLK, G>, dim3(static_cast<unsigned>((2 * touched + per - 1) / per), c->Hkv, c->B), dim3(kv8_threads(G)), 0, st, *c, kb, vb, \
              pitch[0], pitch[1], pitch[2], pitch[3], pitch[4], pitch[5], start, counts, n, err); \
     break; \
   }

@@ -29,7 +29,8 @@
 // Measured with the joining kernel: 32 sequences of 4096 keys, 32 heads of 96 keep 6.6 TB/s (6.5 with dim 64, 6.3 to 6.7 with 128).  8 sequences of
 // 2001 to 4001 keys, 55 heads of 96: 44.5 us, 5.7 TB/s; 65501 and shorter keys, 8 heads of 128 for 32: 41.3 us, 5.0 TB/s, of which finding the
 // shares and the first codes take 4 and joining 4.5.  Five drafted tokens, 16 sequences of up to 6007 keys, 8 heads of 64 for 32: 29.7 us; with
-// 20 rows a step is 700 instructions, and thirteen steps to a warp do not hide them.  512 keys of one sequence: 7.1 us, all latency.
+// 20 rows a step is 565 instructions, in chains that eight warps to an SM do not cover (40 % of the issue slots).  Issuing a step's score products
+// beside the weights of the step before did not help (30.7).  512 keys of one sequence: 7.1 us, all latency.
 #include "kv8.cuh"
 #include "softmax_math.cuh"
 
