@@ -30,7 +30,11 @@
 // 2001 to 4001 keys, 55 heads of 96: 44.5 us, 5.7 TB/s; 65501 and shorter keys, 8 heads of 128 for 32: 41.3 us, 5.0 TB/s, of which finding the
 // shares and the first codes take 4 and joining 4.5.  Five drafted tokens, 16 sequences of up to 6007 keys, 8 heads of 64 for 32: 29.7 us; with
 // 20 rows a step is 565 instructions, in chains that eight warps to an SM do not cover (40 % of the issue slots).  Issuing a step's score products
-// beside the weights of the step before did not help (30.7).  512 keys of one sequence: 7.1 us, all latency.
+// beside the weights of the step before did not help (30.7).  Short ranges are left whole, one to a CTA:
+// 512 keys of one sequence, 55 heads of 96: 6.6 us, all latency (7.2 divided and joined by a second kernel).
+#include <algorithm>
+#include <type_traits>
+
 #include "kv8.cuh"
 #include "softmax_math.cuh"
 
@@ -51,6 +55,7 @@ struct Kv8Attn {
   float scale_log2;
   int ctas;
   uint32_t group_magic;              // ceil(2^32 / group)
+  int whole;                         // ranges are not divided between shares: each counts as one step of one, a warp's (1) or a CTA's (KA_WARPS)
 };
 
 constexpr int KA_WARPS = 4, KA_STEP = 32;           // keys per warp and step
@@ -105,15 +110,16 @@ struct Shares {
     const int b = c + (threadIdx.x & 31);
     len = b < p.B ? min(max(__ldg(p.lens + b), 0), p.most) : 0;
   }
-  __device__ __forceinline__ static uint32_t steps(int n) { return max(1, (n + KA_STEP - 1) / KA_STEP); }      // of a range; without keys it has an empty one
-  __device__ __forceinline__ uint32_t mine(const Kv8Attn& p) const { return chunk + static_cast<int>(threadIdx.x & 31) < p.B ? steps(len) : 0u; }
+  // of a range; without keys it has an empty one
+  __device__ __forceinline__ static uint32_t steps(const Kv8Attn& p, int n) { return p.whole ? 1 : max(1, (n + KA_STEP - 1) / KA_STEP); }
+  __device__ __forceinline__ uint32_t mine(const Kv8Attn& p) const { return chunk + static_cast<int>(threadIdx.x & 31) < p.B ? steps(p, len) : 0u; }
   __device__ __forceinline__ Shares(const Kv8Attn& p) : total(0), per_unit(p.Hkv * p.tiles_r) {
     for (int c = 0; c < p.B; c += 32) {
       load(p, c);
       total += __reduce_add_sync(0xffffffffu, mine(p));
     }
     total *= per_unit;
-    G = min(static_cast<uint32_t>(KA_WARPS * p.ctas), total);
+    G = min(static_cast<uint32_t>(p.whole == KA_WARPS ? p.ctas : KA_WARPS * p.ctas), total);
     each = total / G;
     more = total - each * G;
   }
@@ -165,18 +171,24 @@ struct Range {
   bool begins, ends;                                // the range begins (ends) in this share
   __device__ __forceinline__ void next(const Kv8Attn& p, Shares& sh, uint32_t hi) {
     len = sh.length(p, b);
-    uint32_t n = Shares::steps(len);
+    uint32_t n = Shares::steps(p, len);
     if (step >= base + n * sh.per_unit) {
       base += n * sh.per_unit;
       len = sh.length(p, ++b);
-      n = Shares::steps(len);
+      n = Shares::steps(p, len);
     }
     const uint32_t unit = (step - base) / n, s0 = (step - base) - unit * n, s1 = min(n, s0 + (hi - step));
     step += s1 - s0;
     h = p.tiles_r == 1 ? unit : unit / static_cast<uint32_t>(p.tiles_r);
     r0 = (unit - h * p.tiles_r) * p.rows;
-    key0 = s0 * KA_STEP;
-    key1 = min(static_cast<uint32_t>(len), s1 * KA_STEP);
+    if (p.whole) {                                  // the CTA's warps divide the range's steps
+      const uint32_t all = max(1, (len + KA_STEP - 1) / KA_STEP), w = p.whole == 1 ? 0 : threadIdx.x >> 5;
+      key0 = all * w / p.whole * KA_STEP;
+      key1 = min(static_cast<uint32_t>(len), all * (w + 1) / p.whole * KA_STEP);
+    } else {
+      key0 = s0 * KA_STEP;
+      key1 = min(static_cast<uint32_t>(len), s1 * KA_STEP);
+    }
     begins = s0 == 0;
     ends = s1 == n;
   }
@@ -201,7 +213,8 @@ __host__ __device__ constexpr int kv8_warp_bytes() {        // shared memory of 
   return Kv8Ring<D, NT>::STAGES * Kv8Ring<D, NT>::STAGE + (NT > 1 ? NT * (D / 32) * 32 * 16 + 8 * NT * 4 : 0) + 4 * D;
 }
 
-template <int D, int NT>
+// TOGETHER: a range belongs to a CTA, whose warps divide its steps and join their parts.
+template <int D, int NT, bool TOGETHER>
 __global__ void __launch_bounds__(32 * KA_WARPS, NT > 1 || D == 128 ? 2 : 3)
 kv8_attention_kernel(const Kv8Attn p) {
   using Ring = Kv8Ring<D, NT>;
@@ -218,7 +231,7 @@ kv8_attention_kernel(const Kv8Attn p) {
   pdl_trigger();                                    // behind the wait: the joining kernel may read the lengths at once
   extern __shared__ __align__(16) uint8_t smem[];   // per warp: ring; (NT > 1) q's fragments, factors of its scores; NaNs noted
   Shares sh(p);
-  const uint32_t worker = warp * p.ctas + blockIdx.x;               // few shares go to different SMs
+  const uint32_t worker = TOGETHER ? blockIdx.x : warp * p.ctas + blockIdx.x;         // few shares go to different SMs
   if (worker >= sh.G) return;
   const uint32_t hi = sh.begin(worker + 1);
   Range now, nxt;
@@ -526,7 +539,7 @@ kv8_attention_kernel(const Kv8Attn p) {
     }
 
     // ---- the range's outputs, or this share's part of them
-    const bool whole = now.begins && now.ends;
+    const bool whole = now.begins && now.ends && !TOGETHER;
     noted = __any_sync(0xffffffffu, noted);
 #pragma unroll
     for (int c8 = 0; c8 < NT; ++c8)
@@ -555,7 +568,7 @@ kv8_attention_kernel(const Kv8Attn p) {
               to[16 * w + 8] = f2bf(o[w][c8][i + 2] * e * f);
             }
           } else {
-            float* to = p.part + ((2ll * worker + (now.begins ? 1 : 0)) * p.rows + c) * (D + 4) + g;
+            float* to = p.part + ((TOGETHER ? static_cast<long long>(KA_WARPS) * worker + warp : 2ll * worker + (now.begins ? 1 : 0)) * p.rows + c) * (D + 4) + g;
 #pragma unroll
             for (int w = 0; w < VB; ++w) {
               to[16 * w] = o[w][c8][i];
@@ -570,6 +583,44 @@ kv8_attention_kernel(const Kv8Attn p) {
       for (int d = lane; d < D; d += 32) nan_key[d] = INT_MAX;
       __syncwarp();
     }
+    if constexpr (TOGETHER) {                       // the warps' parts, by way of L2
+      __syncthreads();
+      constexpr int AT_ONCE = NT == 1 ? 2 : 4;      // rows whose loads a warp has in flight
+#pragma unroll 1
+      for (int c0 = warp; c0 < nrows; c0 += AT_ONCE * KA_WARPS) {
+        float2 ml[AT_ONCE][KA_WARPS];
+        float4 v[AT_ONCE][KA_WARPS];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+          for (int w = 0; w < KA_WARPS; ++w) {
+            const int c = min(c0 + KA_WARPS * i, nrows - 1);
+            const float* from = p.part + ((static_cast<long long>(KA_WARPS) * worker + w) * p.rows + c) * (D + 4);
+            ml[i][w] = *reinterpret_cast<const float2*>(from + D);
+            v[i][w] = lane < D / 4 ? *reinterpret_cast<const float4*>(from + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int c = c0 + KA_WARPS * i;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float top = KA_NEG, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < KA_WARPS; ++w) top = fmaxf(top, ml[i][w].x);
+#pragma unroll
+          for (int w = 0; w < KA_WARPS; ++w) {
+            const float half = ex2_approx(0.5f * (ml[i][w].x - top)), f = half * half;
+            sum += ml[i][w].y * half * half;
+            acc.x = fmaf(v[i][w].x, f, acc.x); acc.y = fmaf(v[i][w].y, f, acc.y); acc.z = fmaf(v[i][w].z, f, acc.z); acc.w = fmaf(v[i][w].w, f, acc.w);
+          }
+          const int row = r0 + c, tok = p.n == 1 ? 0 : kv8_token(p, row), hq = now.h * p.group + row - tok * p.group;
+          const float f = sum == 0.f ? 0.f : 1.f / sum, e = pow2i(KA_MID);
+          if (c < nrows && lane < D / 4)
+            *reinterpret_cast<uint2*>(p.out + ((static_cast<size_t>(now.b) * p.n + tok) * p.Hkv * p.group + hq) * D + 4 * lane) =
+                make_uint2(pack_bf16x2(acc.x * e * f, acc.y * e * f), pack_bf16x2(acc.z * e * f, acc.w * e * f));
+        }
+      }
+      __syncthreads();
+    }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -583,7 +634,7 @@ kv8_join_kernel(const Kv8Attn p) {
   __shared__ float4 sm[WARPS][D / 4];
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, idx = blockIdx.x * (WARPS / WR) + warp / WR, place = warp % WR;
   Shares sh(p);                                     // the lengths were there before the kernel above began
-  const uint32_t base = sh.base(p, b), n = Shares::steps(sh.length(p, b));
+  const uint32_t base = sh.base(p, b), n = Shares::steps(p, sh.length(p, b));
   const int unit = idx / p.rows, r = idx - unit * p.rows;
   const int h = unit / p.tiles_r, row = (unit - h * p.tiles_r) * p.rows + r;
   const bool mine = n > 1 && unit < static_cast<int>(sh.per_unit) && row < p.n * p.group;
@@ -646,9 +697,9 @@ kv8_join_kernel(const Kv8Attn p) {
       make_uint2(pack_bf16x2(acc.x * e * f, acc.y * e * f), pack_bf16x2(acc.z * e * f, acc.w * e * f));
 }
 
-template <int D, int NT>
+template <int D, int NT, bool TOGETHER>
 static int kv8_slots() {                            // CTAs that one SM holds
-  auto kern = kv8_attention_kernel<D, NT>;
+  auto kern = kv8_attention_kernel<D, NT, TOGETHER>;
   constexpr int smem = KA_WARPS * kv8_warp_bytes<D, NT>();
   int dev = 0, per = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
@@ -665,10 +716,10 @@ static int kv8_slots() {                            // CTAs that one SM holds
 template <int D>
 static int kv8_slots_d(int nt) {
   switch (nt) {
-    case 1: return kv8_slots<D, 1>();
-    case 2: return kv8_slots<D, 2>();
-    case 3: return kv8_slots<D, 3>();
-    case 4: return kv8_slots<D, 4>();
+    case 1: return std::min(kv8_slots<D, 1, false>(), kv8_slots<D, 1, true>());
+    case 2: return std::min(kv8_slots<D, 2, false>(), kv8_slots<D, 2, true>());
+    case 3: return std::min(kv8_slots<D, 3, false>(), kv8_slots<D, 3, true>());
+    case 4: return std::min(kv8_slots<D, 4, false>(), kv8_slots<D, 4, true>());
     default: return 0;
   }
 }
@@ -700,10 +751,19 @@ static void kv8_join(const Kv8Attn& p, cudaStream_t st) {
 template <int D>
 static void kv8_run(const Kv8Attn& p, int nt, cudaStream_t st) {
   const dim3 block(32 * KA_WARPS), grid(p.ctas);
-  if (nt == 1) launch_k(kv8_attention_kernel<D, 1>, grid, block, KA_WARPS * kv8_warp_bytes<D, 1>(), st, p);
-  else if (nt == 2) launch_k(kv8_attention_kernel<D, 2>, grid, block, KA_WARPS * kv8_warp_bytes<D, 2>(), st, p);
-  else if (nt == 3) launch_k(kv8_attention_kernel<D, 3>, grid, block, KA_WARPS * kv8_warp_bytes<D, 3>(), st, p);
-  else launch_k(kv8_attention_kernel<D, 4>, grid, block, KA_WARPS * kv8_warp_bytes<D, 4>(), st, p);
+  auto run = [&](auto columns, auto together) {
+    constexpr int NT = decltype(columns)::value;
+    launch_k(kv8_attention_kernel<D, NT, decltype(together)::value>, grid, block, KA_WARPS * kv8_warp_bytes<D, NT>(), st, p);
+  };
+  auto pick = [&](auto together) {
+    if (nt == 1) run(std::integral_constant<int, 1>(), together);
+    else if (nt == 2) run(std::integral_constant<int, 2>(), together);
+    else if (nt == 3) run(std::integral_constant<int, 3>(), together);
+    else run(std::integral_constant<int, 4>(), together);
+  };
+  if (p.whole == KA_WARPS) pick(std::true_type());
+  else pick(std::false_type());
+  if (p.whole) return;
   // warps per row of a range by the parts that a range has on average, as long as the machine holds them all at a time
   const long long ranges = static_cast<long long>(p.B) * p.Hkv * p.tiles_r, parts = static_cast<long long>(KA_WARPS) * p.ctas / ranges;
   if (parts > 32 && ranges * p.rows <= 256) kv8_join<D, 16>(p, st);
@@ -715,7 +775,16 @@ static void kv8_run(const Kv8Attn& p, int nt, cudaStream_t st) {
 
 using namespace b200;
 
-// How a call is cut.  plan: [0] rows per row tile, [1] row tiles, [2] CTAs, [3] floats of scratch.
+// Ranges of few steps are left whole: the warps of a CTA (KA_WARPS), or where there are more ranges than CTAs a warp (1), go through one of
+// them sooner than a second kernel joins its parts, and a launch is saved.  Divided and whole, us: 55 ranges of 256 keys 6.8 and 5.6, of 1024 8.8 and 9.0;
+// 440 ranges of 256 keys 7.8 and 6.9, of 1024 14.5 and 12.8; two ranges of sixteen rows and 256 keys 6.9 and 7.1, 512 keys 6.8 and 8.8;
+// 1024 ranges of 128 keys 8.7 and (1) 6.7.
+static int kv8_whole(long long ranges, int most, long long slots) {
+  const int steps = (most + KA_STEP - 1) / KA_STEP;
+  return ranges <= slots && steps <= (ranges < 16 ? 12 : 32) ? KA_WARPS : steps <= 6 ? 1 : 0;
+}
+
+// How a call is cut.  plan: [0] rows per row tile, [1] row tiles, [2] CTAs, [3] floats of scratch, [4] whole ranges.
 B200_API int b200_kv8_attention_plan(int B, int Hkv, int D, int rows, int most, int* plan) {
   if (B <= 0 || B > 65535 || Hkv <= 0 || rows <= 0 || most <= 0) return -1;
   const int tiles_r = (rows + 31) / 32, per = (rows + tiles_r - 1) / tiles_r;
@@ -725,15 +794,17 @@ B200_API int b200_kv8_attention_plan(int B, int Hkv, int D, int rows, int most, 
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -3;
   const long long steps = static_cast<long long>(B) * Hkv * tiles_r * ((static_cast<long long>(most) + KA_STEP - 1) / KA_STEP);
   if (steps > (1ll << 31) - 1 || static_cast<long long>(Hkv) * tiles_r * per > (1ll << 31) - 4) return -4;
-  const long long ctas = steps < static_cast<long long>(sms) * slots ? steps : static_cast<long long>(sms) * slots;
+  const long long ranges = static_cast<long long>(B) * Hkv * tiles_r, most_ctas = static_cast<long long>(sms) * slots;
+  const int whole = kv8_whole(ranges, most, most_ctas);
   plan[0] = per;
   plan[1] = tiles_r;
-  plan[2] = static_cast<int>(ctas);
-  plan[3] = KA_WARPS * plan[2] * 2 * per * (D + 4);
+  plan[2] = static_cast<int>(std::min(whole ? ranges : steps, most_ctas));
+  plan[3] = whole == 1 ? 0 : KA_WARPS * plan[2] * (whole ? 1 : 2) * per * (D + 4);
+  plan[4] = whole;
   return 0;
 }
 
-// a: sizes and cache of the call (rows, tiles_r, ctas and the size of part as planned); the tensors of this call apart from it.
+// a: sizes and cache of the call (rows, tiles_r, ctas, whole and the size of part as planned); the tensors of this call apart from it.
 B200_API int b200_kv8_attention(const Kv8Attn* a, const void* q, const int* lens, void* out, float* part, void* stream) {
   Kv8Attn p = *a;
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -741,8 +812,9 @@ B200_API int b200_kv8_attention(const Kv8Attn* a, const void* q, const int* lens
   p.out = static_cast<__nv_bfloat16*>(out);
   p.part = part;
   if (p.B <= 0 || p.B > 65535 || p.Hkv <= 0 || p.n <= 0 || p.group <= 0 || p.rows <= 0 || p.rows > 32 || p.tiles_r <= 0 || p.ctas <= 0 ||
-      p.log2_block < 4 || p.log2_block > 7 || p.most <= 0 || p.most > p.cap || !p.part)
+      p.log2_block < 4 || p.log2_block > 7 || p.most <= 0 || p.most > p.cap)
     return -1;
+  if ((p.whole != 0 && p.whole != 1 && p.whole != KA_WARPS) || (p.whole != 1 && !p.part)) return -1;
   if (static_cast<long long>(p.rows) * p.tiles_r < static_cast<long long>(p.n) * p.group) return -1;
   if (static_cast<double>(p.n) * p.group * p.group > 4e9) return -4;
   p.group_magic = static_cast<uint32_t>((0x100000000ull + p.group - 1) / p.group);

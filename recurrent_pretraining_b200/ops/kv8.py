@@ -43,7 +43,7 @@ class _Attn(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("k", "v", "ke", "ve")] + [(n, C.c_longlong) for n in ("sb", "sh", "eb", "eh")] + \
                [(n, C.c_int) for n in ("B", "Hkv", "cap", "D", "log2_block")] + [("q", C.c_void_p)] + \
                [(n, C.c_longlong) for n in ("q_sb", "q_sn", "q_sh")] + [(n, C.c_void_p) for n in ("lens", "out", "part")] + \
-               [(n, C.c_int) for n in ("n", "group", "rows", "tiles_r", "most")] + [("scale_log2", C.c_float), ("ctas", C.c_int), ("group_magic", C.c_uint32)]
+               [(n, C.c_int) for n in ("n", "group", "rows", "tiles_r", "most")] + [("scale_log2", C.c_float), ("ctas", C.c_int), ("group_magic", C.c_uint32), ("whole", C.c_int)]
 
 
 _fns = None
@@ -297,13 +297,13 @@ def _attention_call(cache, q, lens, scale, max_len):
         return _prompt_call(cache, q, scale, most)
     ok = _aligned(q)
     f, c, device = _k(), cache._c, cache.device
-    plan = (C.c_int * 4)()
+    plan = (C.c_int * 5)()
     rc = _guarded(device, lambda: f.plan(B, cache.kv_heads, D, n * group, most, plan))
     if rc:
         raise RuntimeError(f"kv8_attention_plan failed with code {rc}")
-    rows, tiles_r, ctas, scratch = plan
+    rows, tiles_r, ctas, scratch, whole = plan
     p = _Attn(c.k, c.v, c.ke, c.ve, c.sb, c.sh, c.eb, c.eh, B, c.Hkv, c.cap, D, c.log2_block, 0, *(_pitch(q) if ok else (0, 0, 0)), 0, 0, 0, n, group, rows,
-              tiles_r, most, scale * 1.4426950408889634, ctas)
+              tiles_r, most, scale * 1.4426950408889634, ctas, 0, whole)
     ref_p, check, attn, stream, empty_like = C.byref(p), f.check, f.attn, f.stream, torch.empty_like
     out_like, part_like = (torch.empty(1, dtype=t, device=device).expand(n) for t, n in ((BF16, q.shape), (F32, (scratch,))))
 

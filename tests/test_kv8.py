@@ -345,7 +345,8 @@ def test_attention_takes_views(device):
     assert torch.equal(kv8.attention(q, view, lens), want)
     assert torch.equal(kv8.attention(odd, view, lens), want)
     cut = kv8.attention(q, view, lens, max_len=100)
-    assert torch.equal(cut, kv8.attention(q, view, i32([100, 90], device)))
+    exact, mag, big = attend(q.cpu().double(), values(view, "k"), values(view, "v"), [100, 90], D ** -0.5)       # (a bound may change the order of the sums)
+    assert ((cut.double().cpu() - exact).abs() <= tolerance(exact, mag, big, D, F16_HALF)).all()
     dk, dv = view.decoded()
     assert torch.equal(dk.double().cpu(), values(view, "k").transpose(1, 2)) and torch.equal(dv.double().cpu(), values(view, "v").transpose(1, 2))
     assert kv8.attention(q[:, :0], view, lens).shape == (B, 0, H, D)
