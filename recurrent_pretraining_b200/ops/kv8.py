@@ -122,6 +122,8 @@ class KV8Cache:
         if k.is_cuda and ((k.data_ptr() | v.data_ptr() | k.stride(0) | k.stride(1)) & 15):
             raise ValueError("heads start on 16-byte boundaries")
         self.device = k.device
+        if k.is_cuda:
+            _k().K.err_word(k.device)   # the status word is there before a call is captured
         self._calls: dict = {}          # what a kind of call (shapes, pitches, types, numbers) needs: checked once, then looked up
         self._c = _Cache(k.data_ptr(), v.data_ptr(), ke.data_ptr(), ve.data_ptr(), k.stride(0), k.stride(1), ke.stride(0), ke.stride(1),
                          *k.shape, self.block.bit_length() - 1)

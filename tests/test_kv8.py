@@ -1,6 +1,9 @@
 """The 8-bit key / value cache (``ops/kv8.py``) against statements in 64 bits: the same tests on CPU tensors (plain path) and on the GPU
 (kernels).  Codes and exponents of given bf16 values are exact; tolerances of the rest are sums of the roundings on the way."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -458,6 +461,41 @@ def test_results_repeat_and_do_not_depend_on_the_batch():
     first = kv8.attention(q, cache, lens)
     for _ in range(5):
         assert torch.equal(kv8.attention(q, cache, lens), first)
+
+
+FIRST_CALLS = """
+import torch
+from recurrent_pretraining_b200.ops import kv8
+from recurrent_pretraining_b200.ops.sampling import sample_tokens
+B, H, D, cap = 2, 4, 64, 2048
+cache, other = kv8.KV8Cache.empty(B, H, cap, D, "cuda"), kv8.KV8Cache.empty(B, H, cap, D, "cuda")
+k = torch.randn(B, 1500, H, D, device="cuda").to(torch.bfloat16)
+qkv, logits = torch.randn(B, 3 * H * D, device="cuda"), torch.randn(B, 9000, device="cuda")
+cos, start, pos, lens = torch.ones(cap, D // 2, device="cuda"), *(torch.full((B,), x, dtype=torch.int32, device="cuda") for x in (0, 1500, 1501))
+u = torch.tensor([0.2, 0.7], device="cuda")
+sin = torch.zeros_like(cos)
+
+def step(cache):
+    kv8.append(cache, k, k, start)
+    q = kv8.rope_append(cache, qkv, cos, sin, pos, H)
+    return kv8.attention(q[:, None], cache, lens), kv8.attention(k[:, :200], cache, lens), kv8.attention(q[:, None], cache, lens, max_len=300), sample_tokens(logits, u, top_p=0.9)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step(cache)
+graph.replay()
+want = step(other)
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+pos[1] = cap
+graph.replay()
+from recurrent_pretraining_b200.ops import cuda as K
+assert K.check_device_status() != 0 and K.check_device_status() == 0
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_may_be_captured():
+    subprocess.run([sys.executable, "-c", FIRST_CALLS], check=True, timeout=300, cwd=Path(__file__).parents[1])
 
 
 @pytest.mark.gpu
