@@ -215,7 +215,8 @@ sample_kernel(const SampleParams p) {
     if (key > cut_key || (key == cut_key && idx < cut_idx)) { cut_key = key; cut_idx = idx; }
   };
   if (min_p > 0.f) {
-    const double thr = static_cast<double>(mx) + static_cast<double>(T_) * log(static_cast<double>(min_p));
+    // an infinite temperature drops nothing that weighs something (and inf - inf would be no threshold)
+    const double thr = isinf(T_) ? -INFINITY : static_cast<double>(mx) + static_cast<double>(T_) * log(static_cast<double>(min_p));
     float f = static_cast<float>(thr);
     uint32_t k = sp_key(f + 0.f);
     if (static_cast<double>(f) < thr) ++k;          // the least float that is not below

@@ -426,7 +426,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     xs, order = torch.sort(x, dim=-1, descending=True, stable=True)
     top = xs[:, :1]
     d = torch.where(xs == top, 0.0, top - xs)
-    w = torch.exp(-torch.where(d > 0, d / torch.where(t > 0, t, 1.0), 0.0))
+    d = torch.where(torch.isinf(d), math.inf, torch.where(d > 0, d / torch.where(t > 0, t, 1.0), 0.0))      # an infinite distance stays one at any t
+    w = torch.exp(-d)
     keep = (k <= 0) | (xs >= xs.gather(1, k.clamp(1, V) - 1))
     prefix = w.cumsum(-1) <= p * w.sum(-1, keepdim=True)
     prefix[:, 0] = True

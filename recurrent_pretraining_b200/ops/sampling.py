@@ -51,7 +51,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     1: off) keeps the longest prefix of the descending order (equal logits: lowest index first) whose probabilities sum to at most
     ``top_p`` and at least one token, ``min_p`` (0: off) drops what has less than ``min_p`` times the largest probability.  Every setting is a number
     or a tensor with one value per row (fp32, ``top_k`` int32).  A ``temperature`` of 0 picks the largest logit, the lowest index among
-    equal ones.  NaN logits count as -inf; a row without any logit above -inf gives -1."""
+    equal ones; an infinite one weighs all logits alike that are not infinitely far below the largest.  NaN logits count as -inf; a row without any logit above -inf gives -1."""
     key = (logits.shape, logits.stride(), logits.dtype, logits.device, uniform.shape, uniform.stride(), uniform.dtype, uniform.device,
            *(_kind(x) for x in (temperature, top_k, top_p, min_p)))
     call = _calls.get(key)

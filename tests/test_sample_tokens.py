@@ -182,3 +182,28 @@ def test_captured_calls_follow_their_tensors():
         graph.replay()
         rows = x.double().cpu().numpy()
         assert out.tolist() == [oracle(rows[b], float(u[b]), 1.0, int(k[b]), float(p[b]), 0.0) for b in range(B)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("per_row", [False, True])
+@pytest.mark.parametrize("V", [6, 20011])
+def test_an_infinite_temperature_weighs_finite_logits_alike(device, per_row, V):
+    """The limit of high temperatures: weight 1, or 0 at an infinite distance from the largest."""
+    inf = float("inf")
+    x = torch.randn(3, V, generator=torch.Generator().manual_seed(2))
+    x[0, 1] = x[1, ::2] = x[1, 5] = -inf
+    x[2, [3, V - 2]] = inf
+    t = torch.full((3,), inf, device=device) if per_row else inf
+    for u in (0.0, 0.1, 0.5, 0.99):
+        for setting in (dict(), dict(min_p=0.3), dict(min_p=1.0), dict(top_k=2), dict(top_p=0.5), dict(top_p=0.5, min_p=1.0)):
+            got = sample_tokens(x.to(device), torch.full((3,), u, device=device), temperature=t, **setting).tolist()
+            for b in range(3):
+                w = (x[b] == inf if b == 2 else x[b] > -inf).numpy()
+                order = np.lexsort((np.arange(V), -x[b].numpy()))
+                keep = w.copy()
+                if "top_k" in setting:
+                    keep &= x[b].numpy() >= x[b].numpy()[order[1]]
+                if "top_p" in setting:
+                    keep[order[max(1, int(0.5 * w.sum())):]] = False
+                kept = np.nonzero(keep)[0]
+                assert got[b] == kept[int(float(np.float32(u)) * kept.size)], (u, setting, b)
