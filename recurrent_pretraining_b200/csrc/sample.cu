@@ -104,11 +104,11 @@ __device__ __forceinline__ void sp_add(SampleHist& h, int bin, unsigned long lon
 __device__ __forceinline__ unsigned long long sp_mass(const SampleHist& h, int bin) { return *reinterpret_cast<const unsigned long long*>(&h.mass[bin]); }
 
 struct SampleScale {
-  float mx, cf;
+  float mx;
   double c, mxc;                                    // log2(e) / T; max times that
 };
 // 2^-y, y = (max - v) log2(e) / T = a + i / 256 + r, in units of 2^-44.
-__device__ __forceinline__ unsigned long long sp_weight_inline(float v, float mx, float cf, double c, double mxc, const double* tab) {
+__device__ __forceinline__ unsigned long long sp_weight_inline(float v, float mx, double c, double mxc, const double* tab) {
   const double y = fma(-static_cast<double>(v), c, mxc);
   const double big = 6755399441055744.0 / SP_TAB;   // 1.5 * 2^52 / 256: adding it leaves round(256 y) in the low bits
   const double z = y + big;
@@ -117,12 +117,12 @@ __device__ __forceinline__ unsigned long long sp_weight_inline(float v, float mx
   const double e = fma(r, fma(r, fma(r, -0.055504108664821580, 0.24022650695910071), -0.69314718055994531), 1.0);
   const double f = fma(tab[q & (SP_TAB - 1)], e, 4503599627370496.0);           // 2^52: the low bits are the rounded integer
   const unsigned long long w = (static_cast<unsigned long long>(__double_as_longlong(f)) & 0xFFFFFFFFFFFFFull) >> (q >> 8 & 63);
-  return v == mx ? 1ull << SP_ONE : (mx - v) * cf < SP_ONE + 1.f ? w : 0ull;    // (infinities, too)
+  return v == mx ? 1ull << SP_ONE : y < SP_ONE + 1. ? w : 0ull;     // (infinities, too; y because mx - v and c may leave fp32)
 }
 // Not inlined where speed does not ask for it: a row runs through every stage of the kernel once, and with eight copies of this in it the
 // fetching of instructions took a third of its time.
-__device__ __noinline__ unsigned long long sp_weight(float v, float mx, float cf, double c, double mxc, const double* tab) {
-  return sp_weight_inline(v, mx, cf, c, mxc, tab);
+__device__ __noinline__ unsigned long long sp_weight(float v, float mx, double c, double mxc, const double* tab) {
+  return sp_weight_inline(v, mx, c, mxc, tab);
 }
 static_assert(SP_TAB == 256, "shifts by eight above");
 
@@ -203,10 +203,9 @@ sample_kernel(const SampleParams p) {
   SampleScale sc;
   sc.mx = mx;
   sc.c = 1.4426950408889634 / static_cast<double>(T_);
-  sc.cf = static_cast<float>(sc.c);
   sc.mxc = static_cast<double>(mx) * sc.c;
-  const float cf = sc.cf;
-  auto weight = [&](float v) { return sp_weight(v, sc.mx, sc.cf, sc.c, sc.mxc, s.tab); };
+  const float cf = static_cast<float>(sc.c);        // for bins, which do not have to be exact
+  auto weight = [&](float v) { return sp_weight(v, sc.mx, sc.c, sc.mxc, s.tab); };
 
   // ---- the cut: kept are keys above cut_key, and those equal to it with an index up to cut_idx
   uint32_t cut_key = 0;
@@ -273,7 +272,7 @@ sample_kernel(const SampleParams p) {
       for (int i = w0 + lane; i < w1; i += 32) {
         const float v = at(i);
         const int bin = bin_of(v);
-        const unsigned long long w = by_p ? sp_weight_inline(v, sc.mx, sc.cf, sc.c, sc.mxc, s.tab) : 0ull;
+        const unsigned long long w = by_p ? sp_weight_inline(v, sc.mx, sc.c, sc.mxc, s.tab) : 0ull;
         if (bin == SP_BINS - 1) {
           ++rest;
           rest_w += w;

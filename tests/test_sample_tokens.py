@@ -207,3 +207,19 @@ def test_an_infinite_temperature_weighs_finite_logits_alike(device, per_row, V):
                     keep[order[max(1, int(0.5 * w.sum())):]] = False
                 kept = np.nonzero(keep)[0]
                 assert got[b] == kept[int(float(np.float32(u)) * kept.size)], (u, setting, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("V", [50, 5000])
+@pytest.mark.parametrize("setting", [dict(), dict(p=0.6), dict(k=20), dict(k=30, p=0.4), dict(m=0.1)], ids=str)
+def test_logits_further_apart_than_the_largest_number(device, V, setting):
+    """Distances of more than 3.4e38 under a temperature that makes weights of them."""
+    x = torch.rand(4, V, generator=torch.Generator().manual_seed(12)) * 2 - 1
+    compare(x * 3.4e38, numbers(4, 3), device, t=1e38, **setting)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("setting", [dict(), dict(p=0.6), dict(k=20), dict(m=0.1)], ids=str)
+def test_temperatures_below_the_smallest_normal_number(device, setting):
+    x = torch.rand(4, 3001, generator=torch.Generator().manual_seed(13)) * 1e-38
+    compare(x, numbers(4, 4), device, t=2e-39, **setting)
