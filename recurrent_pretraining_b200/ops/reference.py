@@ -436,7 +436,7 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     kept = torch.zeros_like(w).scatter(1, order, torch.where(keep, w, 0.0)).cumsum(-1)
     u = torch.nan_to_num(uniform.double(), nan=0.0).clamp_min(0.0)
     hit = kept > u[:, None] * kept[:, -1:]
-    last = torch.where(keep, order, -1).amax(-1)         # a number of 1 or more: the last kept token
+    last = torch.where(keep & (d <= 44 * math.log(2.0)), order, -1).amax(-1)         # a number of 1 or more: the last kept token that weighs 2^-44 or more
     token = torch.where(hit.any(-1), hit.int().argmax(-1), last)
     token = torch.where(t[:, 0] > 0, token, order[:, 0])
     return torch.where(top[:, 0] == -math.inf, -1, token)

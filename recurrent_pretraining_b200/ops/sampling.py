@@ -45,7 +45,8 @@ def _setting(x, name: str, logits, dtype, low, high):
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
     """One token (int64) per row of ``logits`` [B, vocab] (bf16 or fp32) from the row's number ``uniform[b]`` in [0, 1) (fp32): the first
     index, in the vocabulary's order, at which the sum of the kept probabilities exceeds ``uniform`` times their total (a number below 0 or
-    NaN counts as 0, one of 1 or more gives the last kept token).
+    NaN counts as 0, one of 1 or more gives the last kept token that has a weight: what has less than 2^-44
+    of the largest probability is never drawn).
 
     Kept is what all filters keep, as in ``models.sampling``: ``top_k`` (0: off) drops what is below the k-th largest logit, ``top_p`` (0 or
     1: off) keeps the longest prefix of the descending order (equal logits: lowest index first) whose probabilities sum to at most

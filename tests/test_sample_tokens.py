@@ -223,3 +223,18 @@ def test_logits_further_apart_than_the_largest_number(device, V, setting):
 def test_temperatures_below_the_smallest_normal_number(device, setting):
     x = torch.rand(4, 3001, generator=torch.Generator().manual_seed(13)) * 1e-38
     compare(x, numbers(4, 4), device, t=2e-39, **setting)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("V", [4, 9000])
+def test_numbers_from_one_on_take_the_last_kept_token_with_a_weight(device, V):
+    """Tokens below 2^-44 of the largest weigh nothing and are never drawn."""
+    x = torch.full((4, V), -2000.0)
+    x[:, 0], x[:, 1], x[:, 2] = 5.0, 0.0, -200.0
+    x[2, V - 1] = 5 - 30.0                  # e^-30 = 2^-43.3
+    x[3, V - 1] = 5 - 31.2                  # 2^-45.01
+    for u in (1.0, 7.0, float("inf")):
+        got = sample_tokens(x.to(device), torch.full((4,), u, device=device)).tolist()
+        assert got == [1, 1, V - 1, 1]
+        assert sample_tokens(x.to(device), torch.full((4,), u, device=device), top_k=1).tolist() == [0] * 4
+        assert sample_tokens(x.to(device), torch.full((4,), u, device=device), temperature=1000.0).tolist() == [V - 1] * 4
