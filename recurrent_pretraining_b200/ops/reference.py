@@ -432,7 +432,7 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     prefix = w.cumsum(-1) <= p * w.sum(-1, keepdim=True)
     prefix[:, 0] = True
     keep &= prefix | (p <= 0) | (p >= 1)
-    keep &= (m <= 0) | (w >= m)
+    keep &= (m <= 0) | (d <= -torch.log(m))              # by distance: weights near 1 round to it
     kept = torch.zeros_like(w).scatter(1, order, torch.where(keep, w, 0.0)).cumsum(-1)
     u = torch.nan_to_num(uniform.double(), nan=0.0).clamp_min(0.0)
     hit = kept > u[:, None] * kept[:, -1:]

@@ -238,3 +238,13 @@ def test_numbers_from_one_on_take_the_last_kept_token_with_a_weight(device, V):
         assert got == [1, 1, V - 1, 1]
         assert sample_tokens(x.to(device), torch.full((4,), u, device=device), top_k=1).tolist() == [0] * 4
         assert sample_tokens(x.to(device), torch.full((4,), u, device=device), temperature=1000.0).tolist() == [V - 1] * 4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_min_p_of_one_keeps_the_largest_alone(device):
+    """However close the next one is: its weight is below the largest's, although the difference is lost when weights are numbers near one."""
+    x = torch.full((2, 3000), -5.0)
+    x[0, [10, 2000]] = torch.tensor([1e-30, 2e-30])
+    x[1, [10, 2000, 2500]] = torch.tensor([4.0, 4.0, 3.9999998])
+    for u, want in ((0.0, [2000, 10]), (0.4, [2000, 10]), (0.9, [2000, 2000])):
+        assert sample_tokens(x.to(device), torch.full((2,), u, device=device), min_p=1.0).tolist() == want
