@@ -306,15 +306,18 @@ class DecodeEngine(GraphRunner):
 
     @torch.no_grad()
     def prefill(self, input_ids: torch.Tensor, num_steps: int | None = None, init_scale: float = 1.0,
-                sampling: SamplingOptions | None = None):
+                sampling: SamplingOptions | None = None, generator: torch.Generator | None = None):
         """Process the prompt with the ordinary (large-M) kernels, filling every cache slot; returns the first
-        generated token and the last-position latent."""
+        generated token, drawn from new numbers of ``generator`` where ``sampling`` says so."""
         B, P = input_ids.shape
         assert B == self.B, "engine was built for a fixed batch"
+        sampled = self._settings(sampling)
+        if sampled:
+            self.uniform.uniform_(generator=generator)
         self.cache._seen_tokens = 0
         out = self.model(input_ids, num_steps=num_steps or self.r, use_cache=True, past_key_values=self.cache,
                          cache_position=torch.arange(P, device=self.dev), init_scale=init_scale)
-        self.tok.copy_(self._pick(out.logits[:, -1, :], self._settings(sampling)))
+        self.tok.copy_(self._pick(out.logits[:, -1, :], sampled))
         self.state.copy_(out.latent_states[:, -1, :])
         self.pos.fill_(P)
         self.lens.fill_(P + 1)
@@ -345,9 +348,7 @@ class DecodeEngine(GraphRunner):
         sampled = self._settings(sampling)
         if sampled and criterion is not None:
             raise ValueError("sampling goes with a fixed number of recurrences")
-        if sampled:
-            self.uniform.uniform_(generator=generator)
-        first = self.prefill(input_ids, r, init_scale, sampling)
+        first = self.prefill(input_ids, r, init_scale, sampling, generator)
         out = [first]
         steps_log = []
         if criterion is None:

@@ -142,3 +142,25 @@ def test_an_8bit_cache_is_refused_where_there_is_none():
 
     with pytest.raises(ValueError):
         S.make_backend(Tiny(2, 2), kv_dtype="fp8")
+
+
+# Weights of a temperature this high are equal whatever the logits are, so the token is the number's place in the vocabulary: floor(u V).
+FLAT = dict(do_sample=True, temperature=1e30)
+
+
+def places(generator, B, V, steps):
+    return torch.stack([(torch.empty(B, device="cuda").uniform_(generator=generator).double() * V).floor().long() for _ in range(steps)], 1)
+
+
+@gpu
+def test_prefill_draws_from_numbers_of_its_own(model):
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+    from recurrent_pretraining_b200.models.sampling import SamplingOptions
+
+    ids = torch.randint(0, 4000, (2, 20), device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    eng = DecodeEngine(model, max_batch=2, max_len=64, num_steps=4)
+    flat = SamplingOptions(**FLAT)
+    first, second = (eng.prefill(ids, init_scale=0.0, sampling=flat) for _ in range(2))
+    assert not torch.equal(first, second)
+    drawn = eng.prefill(ids, init_scale=0.0, sampling=flat, generator=torch.Generator("cuda").manual_seed(3))
+    assert torch.equal(drawn, places(torch.Generator("cuda").manual_seed(3), 2, eng.V, 1)[:, 0])
