@@ -293,10 +293,10 @@ class DecodeEngine(GraphRunner):
             return False
         if sampling.repetition_penalty not in (None, 1.0):
             raise ValueError("the recurrent decode engine has no repetition penalty")
-        given = dict(temperature=float(sampling.temperature or 1.0), top_k=int(sampling.top_k or 0), top_p=float(sampling.top_p or 1.0),
+        given = dict(temperature=1.0 if sampling.temperature is None else float(sampling.temperature), top_k=int(sampling.top_k or 0), top_p=float(sampling.top_p or 1.0),
                      min_p=float(sampling.min_p or 0.0))
-        if not (given["temperature"] > 0 and 0 <= given["top_k"] < 2 ** 31 and 0 <= given["top_p"] <= 1 and 0 <= given["min_p"] <= 1):
-            raise ValueError(f"sampling needs temperature > 0, top_k >= 0, top_p and min_p in 0 .. 1: got {given}")
+        if not (given["temperature"] >= 0 and 0 <= given["top_k"] < 2 ** 31 and 0 <= given["top_p"] <= 1 and 0 <= given["min_p"] <= 1):
+            raise ValueError(f"sampling needs temperature >= 0, top_k >= 0, top_p and min_p in 0 .. 1: got {given}")
         for name, x in given.items():
             self.sampling[name].fill_(x)
         return True

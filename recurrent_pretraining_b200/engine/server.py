@@ -53,8 +53,11 @@ class DecodeOptions:
                 self.continuous_compute, self.init_scale, *self.sampling().items())
 
     def sampling(self) -> dict:
-        """The sampling options that are set."""
-        return {k: getattr(self, k) for k in self.SAMPLING if getattr(self, k) not in (None, False)}
+        """The sampling options that are set; a temperature of 0 is greedy decoding, whatever the model is."""
+        given = {k: getattr(self, k) for k in self.SAMPLING if getattr(self, k) not in (None, False)}
+        if self.temperature is not None and self.temperature == 0:
+            given.pop("do_sample", None)
+        return given
 
 
 @dataclass

@@ -164,3 +164,37 @@ def test_prefill_draws_from_numbers_of_its_own(model):
     assert not torch.equal(first, second)
     drawn = eng.prefill(ids, init_scale=0.0, sampling=flat, generator=torch.Generator("cuda").manual_seed(3))
     assert torch.equal(drawn, places(torch.Generator("cuda").manual_seed(3), 2, eng.V, 1)[:, 0])
+
+
+def test_a_request_with_a_temperature_of_zero_is_greedy():
+    from recurrent_pretraining_b200.engine import server as S
+
+    cold, none = S.DecodeOptions(do_sample=True, temperature=0.0), S.DecodeOptions(do_sample=True)
+    assert cold.sampling() == {} and none.sampling() == {"do_sample": True}
+    assert cold.key() != none.key() and cold.key() == S.DecodeOptions().key()
+    off = S.DecodeOptions(do_sample=True, temperature=0.7, top_k=0, top_p=0.0, min_p=0.0)                  # filters of zero are off, as if not given
+    assert off.sampling() == {"do_sample": True, "temperature": 0.7}
+
+
+@gpu
+def test_a_temperature_of_zero_takes_the_largest_logit(model):
+    """As ``sample_tokens`` does: not a draw at another temperature."""
+    from recurrent_pretraining_b200.engine import server as S
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+    from recurrent_pretraining_b200.models.sampling import SamplingOptions
+
+    ids = torch.randint(0, 4000, (2, 20), device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    eng = DecodeEngine(model, max_batch=2, max_len=64, num_steps=4)
+    cold = SamplingOptions(do_sample=True, temperature=0.0)
+    logits = torch.randn(2, 4096, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    logits[1, [7, 4000]] = 9.0
+    eng.uniform.fill_(0.75)
+    assert torch.equal(eng._pick(logits, eng._settings(cold)), torch.stack([logits[0].argmax(), torch.tensor(7, device="cuda")]))
+    assert nearly_largest(model, eng.generate(ids, 10, init_scale=0.0, sampling=cold)[0], 20)
+    sched = S.BatchScheduler(S.make_backend(model, max_batch=2, max_len=64), window_ms=5.0, stop_ids=())
+    try:
+        body = {"prompt": [5, 17, 3], "max_tokens": 8, "num_steps": 4, "init_scale": 0.0, "do_sample": True, "temperature": 0}
+        tokens = S.handle_completion(sched, body)["choices"][0]["token_ids"]
+        assert nearly_largest(model, torch.tensor([body["prompt"] + tokens], device="cuda"), 3)
+    finally:
+        sched.close()
