@@ -31,6 +31,8 @@ from ..ops.reference import KV8_EMIN
 from ..ops.sampling import sample_tokens
 from .base import BF16, PDL, SKINNY_ROWS, GraphRunner, skinny_linear
 
+BAD_INDEX = 8      # device status: a token outside its table
+
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
 _swiglu_acc = K._sig("b200_swiglu_acc", [_vp, _vp, C.c_longlong, _i, _vp])
 _norm_pair = K._sig("b200_add_rmsnorm_pair", [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _f, _vp])
@@ -341,7 +343,8 @@ class DecodeEngine(GraphRunner):
                  sampling: SamplingOptions | None = None, generator: torch.Generator | None = None):
         """Decoding, greedy unless ``sampling`` says otherwise.  ``criterion=None``: fixed ``num_steps`` recurrences per token.
         ``criterion="kl"``: KL exit with ``exit_threshold`` and at most ``max_steps`` recurrences (greedy only).  Sampled tokens are
-        drawn from uniform numbers of ``generator`` (a generator of the engine's device).  Returns (tokens [B, P+new], stats)."""
+        drawn from uniform numbers of ``generator`` (a generator of the engine's device); a row without a finite logit gives -1, which the
+        device status reports.  Returns (tokens [B, P+new], stats)."""
         r = num_steps or self.r
         B, P = input_ids.shape
         assert P + max_new_tokens <= self.Lmax
@@ -373,7 +376,10 @@ class DecodeEngine(GraphRunner):
                                                 min_steps))
                 steps_log.append(self.steps_taken.tolist())
         tokens = torch.cat([input_ids, torch.stack(out, dim=1)], dim=1)
-        return tokens, {"steps": steps_log, "device_status": K.check_device_status()}
+        status = K.check_device_status()
+        if sampled and not status and bool((tokens[:, P:] < 0).any()):     # a row without a finite logit; a last token is not looked up by a later step
+            status = BAD_INDEX
+        return tokens, {"steps": steps_log, "device_status": status}
 
     def _token_adaptive(self, cap, threshold, init_scale, continuous, check_every, min_steps):
         B = self.B

@@ -198,3 +198,30 @@ def test_a_temperature_of_zero_takes_the_largest_logit(model):
         assert nearly_largest(model, torch.tensor([body["prompt"] + tokens], device="cuda"), 3)
     finally:
         sched.close()
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 3])
+def test_rows_without_a_finite_logit_are_reported(model, new):
+    """Also where the token is the last one of a request, which no later step looks up."""
+    from recurrent_pretraining_b200.engine import server as S
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+    from recurrent_pretraining_b200.models.sampling import SamplingOptions
+
+    ids = torch.randint(0, 4000, (2, 12), device="cuda", generator=torch.Generator("cuda").manual_seed(6))
+    hot = SamplingOptions(do_sample=True, temperature=1.0)
+    eng = DecodeEngine(model, max_batch=2, max_len=32, num_steps=4)
+    keep = model.lm_head.weight.detach().clone()
+    try:
+        with torch.no_grad():
+            model.lm_head.weight.fill_(float("nan"))
+        _, stats = eng.generate(ids, new, init_scale=0.0, sampling=hot)
+        assert stats["device_status"] != 0
+        backend = S.make_backend(model, max_batch=1, max_len=32)
+        with pytest.raises(RuntimeError):
+            backend.generate([[5, 17, 3]], S.DecodeOptions(max_tokens=new, num_steps=4, init_scale=0.0, do_sample=True))
+    finally:
+        with torch.no_grad():
+            model.lm_head.weight.copy_(keep)
+    tokens, stats = eng.generate(ids, new, init_scale=0.0, sampling=hot)
+    assert stats["device_status"] == 0 and (tokens >= 0).all()
