@@ -13,6 +13,8 @@
 // Appending is bound by memory: 4 x 1024 tokens of 55 heads of 96 take 22.0 us, 5.9 TB/s of reads and writes mixed (28.1 with the magnitudes
 // compared as fp32 numbers: there were more instructions than the memory left time for).  A step's tokens (64 sequences, 48
 // heads of 128) take 2.6 us, about an empty launch.
+#include <algorithm>
+
 #include "kv8.cuh"
 
 namespace b200 {
@@ -260,9 +262,10 @@ kv8_tiles_kernel(const int* __restrict__ lens, int4* __restrict__ tiles, __nv_bf
     for (int x = threadIdx.x; x < noted; x += 256) nan_first[static_cast<long long>(b) * noted + x] = INT_MAX;
 }
 
-// A thread per channel of a key head: the outputs [B, n, H, D] of the queries that see its first noted NaN.
+// A thread per channel of a key head: the outputs [B, n, .., D] (pitch `row` per token) of the queries that see its first noted NaN.
 __global__ void __launch_bounds__(128)
-kv8_nan_kernel(const int* __restrict__ nan_first, const int* __restrict__ lens, __nv_bfloat16* __restrict__ out, int n, int group, int Hkv, int D, int most) {
+kv8_nan_kernel(const int* __restrict__ nan_first, const int* __restrict__ lens, __nv_bfloat16* __restrict__ out, int n, int group, int Hkv, int D, int most,
+               long long row) {
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.y, h = blockIdx.x, d = threadIdx.x;
@@ -271,7 +274,7 @@ kv8_nan_kernel(const int* __restrict__ nan_first, const int* __restrict__ lens, 
   if (first == INT_MAX) return;
   const int len = min(max(lens[b], 0), most);
   for (int i = max(0, first - (len - n)); i < n; ++i)
-    for (int x = 0; x < group; ++x) out[((static_cast<long long>(b) * n + i) * Hkv * group + h * group + x) * D + d] = __float2bfloat16(NAN);
+    for (int x = 0; x < group; ++x) out[(static_cast<long long>(b) * n + i) * row + (h * group + x) * D + d] = __float2bfloat16(NAN);
 }
 
 }  // namespace b200
@@ -349,58 +352,99 @@ B200_API int b200_parted_attention(const void* q, const void* k, const void* v, 
                                    int n_tiles, int T, int K, int H, int G, int dim, int vdim, int ld_q, int ld_kv, int ld_out, float scale,
                                    void* stream, int* err);
 
+// Sequences and key heads are answered group by group through the same scratch memory, so that its size does not follow batch and capacity.
 struct Kv8Prompt {
-  int L, per_seq, parts;                          // key rows per sequence, query tiles per sequence, CTAs per tile
+  int L, per_seq;                                 // key rows and query tiles per sequence
+  int seqs, heads;                                // of a group: sequences, key heads
+  size_t bytes;                                   // of scratch memory
+};
+struct Kv8Places {
+  int parts;                                      // CTAs per tile
   size_t v, tiles, nans, refs, sums, bytes;       // places in the scratch memory; keys are first
 };
-static bool kv8_prompt_plan(Kv8Prompt* x, int B, int Hkv, int H, int D, int n, int most) {
+static Kv8Places kv8_prompt_places(const Kv8Prompt& x, int seqs, int heads, int group, int D, int most) {
+  Kv8Places at = {};
+  const long long W = static_cast<long long>(heads) * D, n_tiles = static_cast<long long>(seqs) * x.per_seq, H = static_cast<long long>(heads) * group;
+  at.parts = b200_attention_parts(static_cast<int>(n_tiles), static_cast<int>(H), most);
+  auto place = [&](size_t bytes) { const size_t p = at.bytes; at.bytes += (bytes + 255) & ~size_t(255); return p; };
+  const size_t rows = static_cast<size_t>(seqs) * x.L * W * 2, cells = at.parts > 1 ? static_cast<size_t>(n_tiles) * H * at.parts * 256 : 0;
+  place(rows);
+  at.v = place(rows);
+  at.tiles = place(n_tiles * 16);
+  at.nans = place(static_cast<size_t>(seqs) * W * 4);
+  at.refs = place(cells * 8);
+  at.sums = place(cells * D * 4);
+  return at;
+}
+// Groups that need at most `limit` bytes, or one key head of one sequence.  Whole sequences, as long as there is room: their tiles fill the machine sooner.
+static bool kv8_prompt_plan(Kv8Prompt* x, int B, int Hkv, int H, int D, int n, int most, long long limit) {
+  if (most > INT_MAX - 127 || n > INT_MAX - 255 || static_cast<long long>(H) * D > INT_MAX) return false;
   x->L = (most + 127) & ~127;
   x->per_seq = (n + 255) / 256;
-  const long long W = static_cast<long long>(Hkv) * D, n_tiles = static_cast<long long>(B) * x->per_seq;
-  if (n_tiles > 65535 / 4 || static_cast<long long>(B) * (x->L > n ? x->L : n) >= (1ll << 31) || static_cast<long long>(H) * D >= (1ll << 31)) return false;
-  x->parts = b200_attention_parts(static_cast<int>(n_tiles), H, most);
-  size_t at = 0;
-  auto place = [&](size_t bytes) { const size_t p = at; at += (bytes + 255) & ~size_t(255); return p; };
-  const size_t rows = static_cast<size_t>(B) * x->L * W * 2, cells = x->parts > 1 ? static_cast<size_t>(n_tiles) * H * x->parts * 256 : 0;
-  place(rows);
-  x->v = place(rows);
-  x->tiles = place(n_tiles * 16);
-  x->nans = place(static_cast<size_t>(B) * W * 4);
-  x->refs = place(cells * 8);
-  x->sums = place(cells * D * 4);
-  x->bytes = at;
+  const int fit = std::min((65535 / 4) / x->per_seq, INT_MAX / std::max(x->L, n));       // tiles in a grid, rows in 31 bits
+  if (fit < 1) return false;
+  x->seqs = std::min(B, fit);
+  x->heads = Hkv;
+  auto need = [&] {                               // of the full groups and of those that are left over
+    size_t most_bytes = 0;
+    for (int seqs : {x->seqs, B % x->seqs})
+      for (int heads : {x->heads, Hkv % x->heads})
+        if (seqs && heads) most_bytes = std::max(most_bytes, kv8_prompt_places(*x, seqs, heads, H / Hkv, D, most).bytes);
+    return most_bytes;
+  };
+  while ((x->bytes = need()) > static_cast<size_t>(std::max(limit, 0ll)) && (x->seqs > 1 || x->heads > 1)) {
+    if (x->seqs > 1) x->seqs = (x->seqs + 1) / 2;
+    else x->heads = (x->heads + 1) / 2;
+  }
   return true;
 }
 
-// Bytes of scratch memory; 0: too many tokens for one call.
-B200_API long long b200_kv8_prompt_scratch(int B, int Hkv, int H, int D, int n, int most) {
+// Bytes of scratch memory, at most `limit` where a key head of a sequence does not take more; 0: too many tokens for the attention of tiles.
+B200_API long long b200_kv8_prompt_scratch(int B, int Hkv, int H, int D, int n, int most, long long limit) {
   Kv8Prompt x;
-  if (B <= 0 || Hkv <= 0 || H <= 0 || D <= 0 || n <= 0 || most <= 0 || !kv8_prompt_plan(&x, B, Hkv, H, D, n, most)) return 0;
+  if (B <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || D <= 0 || n <= 0 || most <= 0 || !kv8_prompt_plan(&x, B, Hkv, H, D, n, most, limit)) return 0;
   return static_cast<long long>(x.bytes);
 }
 
 // q, out: bf16 [B, n, H, D] contiguous; no length counts for more than `most`; scratch as above.
-B200_API int b200_kv8_prompt(const Kv8Cache* c, const void* q, const int* lens, void* out, void* scratch, int H, int n, int most, float scale, int* err,
-                             void* stream) {
+B200_API int b200_kv8_prompt(const Kv8Cache* c, const void* q, const int* lens, void* out, void* scratch, int H, int n, int most, float scale,
+                             long long limit, int* err, void* stream) {
   Kv8Prompt x;
-  if (!kv8_cache_ok(c) || H <= 0 || H % c->Hkv || n <= 0 || most <= 0 || most > c->cap || !scratch || !kv8_prompt_plan(&x, c->B, c->Hkv, H, c->D, n, most))
+  if (!kv8_cache_ok(c) || H <= 0 || H % c->Hkv || n <= 0 || most <= 0 || most > c->cap || !scratch ||
+      !kv8_prompt_plan(&x, c->B, c->Hkv, H, c->D, n, most, limit))
     return -1;
   if (reinterpret_cast<uintptr_t>(scratch) & 255) return -2;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int B = c->B, D = c->D, W = c->Hkv * D, n_tiles = B * x.per_seq;
+  const int D = c->D, group = H / c->Hkv;
+  const long long row = static_cast<long long>(H) * D;
   char* mem = static_cast<char*>(scratch);
-  int *tiles = reinterpret_cast<int*>(mem + x.tiles), *nans = reinterpret_cast<int*>(mem + x.nans);
-  launch_k(kv8_tiles_kernel, dim3(B, x.per_seq), dim3(256), 0, st, lens, reinterpret_cast<int4*>(tiles), static_cast<__nv_bfloat16*>(out), n, most, x.L,
-           x.per_seq, static_cast<long long>(H) * D, nans, W);
-  int rc = b200_kv8_decode(c, lens, mem, mem + x.v, x.L, most, nans, n, stream);
-  if (rc) return rc;
-  if (x.parts > 1)
-    rc = b200_parted_attention(q, mem, mem + x.v, out, tiles, mem + x.sums, mem + x.refs, x.parts, n_tiles, B * n, B * x.L, H, c->Hkv, D, D, H * D, W, H * D,
-                               scale, stream, err);
-  else
-    rc = b200_capped_attention(q, mem, mem + x.v, out, tiles, nullptr, n_tiles, B * n, B * x.L, H, c->Hkv, D, D, H * D, W, H * D, 1 << 30, 0, scale, 0.f, 0.f,
-                               stream, err);
-  if (rc) return rc - 100;
-  launch_k(kv8_nan_kernel, dim3(c->Hkv, B), dim3(128), 0, st, nans, lens, static_cast<__nv_bfloat16*>(out), n, H / c->Hkv, c->Hkv, D, most);
+  for (int b0 = 0; b0 < c->B; b0 += x.seqs)
+    for (int h0 = 0; h0 < c->Hkv; h0 += x.heads) {
+      Kv8Cache part = *c;                         // the group's sequences and key heads
+      part.B = std::min(x.seqs, c->B - b0);
+      part.Hkv = std::min(x.heads, c->Hkv - h0);
+      part.k += b0 * c->sb + h0 * c->sh;
+      part.v += b0 * c->sb + h0 * c->sh;
+      part.ke += b0 * c->eb + h0 * c->eh;
+      part.ve += b0 * c->eb + h0 * c->eh;
+      const Kv8Places at = kv8_prompt_places(x, part.B, part.Hkv, group, D, most);
+      const int W = part.Hkv * D, n_tiles = part.B * x.per_seq, heads = part.Hkv * group;
+      int *tiles = reinterpret_cast<int*>(mem + at.tiles), *nans = reinterpret_cast<int*>(mem + at.nans);
+      const __nv_bfloat16* qg = static_cast<const __nv_bfloat16*>(q) + static_cast<long long>(b0) * n * row + static_cast<long long>(h0) * group * D;
+      __nv_bfloat16 *rows = static_cast<__nv_bfloat16*>(out) + static_cast<long long>(b0) * n * row, *og = rows + static_cast<long long>(h0) * group * D;
+      // all heads' outputs of queries without keys become zero with the first group of heads
+      launch_k(kv8_tiles_kernel, dim3(part.B, x.per_seq), dim3(256), 0, st, lens + b0, reinterpret_cast<int4*>(tiles), rows, n, most, x.L, x.per_seq,
+               h0 ? 0ll : row, nans, W);
+      int rc = b200_kv8_decode(&part, lens + b0, mem, mem + at.v, x.L, most, nans, n, stream);
+      if (rc) return rc;
+      if (at.parts > 1)
+        rc = b200_parted_attention(qg, mem, mem + at.v, og, tiles, mem + at.sums, mem + at.refs, at.parts, n_tiles, part.B * n, part.B * x.L, heads, part.Hkv, D,
+                                   D, H * D, W, H * D, scale, stream, err);
+      else
+        rc = b200_capped_attention(qg, mem, mem + at.v, og, tiles, nullptr, n_tiles, part.B * n, part.B * x.L, heads, part.Hkv, D, D, H * D, W, H * D, 1 << 30, 0,
+                                   scale, 0.f, 0.f, stream, err);
+      if (rc) return rc - 100;
+      launch_k(kv8_nan_kernel, dim3(part.Hkv, part.B), dim3(128), 0, st, nans, lens + b0, og, n, group, part.Hkv, D, most, row);
+    }
   return cudaGetLastError() == cudaSuccess ? 0 : -10;
 }

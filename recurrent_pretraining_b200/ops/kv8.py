@@ -23,6 +23,10 @@ from . import reference as ref
 
 BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
 BLOCKS = (16, 32, 64, 128)
+# Bytes of bf16 keys, values and partial sums that a long prompt's attention may hold at a time (one key head of one sequence may take more).
+# Smaller groups leave the machine idle at their ends: 32 sequences of 16384 keys, 8 key heads of 128, 128 tokens of 32 heads take 2054 us
+# all at once, 2073 with 2 GiB, 2186 with 1 and 2559 with a quarter; of 500 keys in that capacity 236, 311, 403 and 542.
+PROMPT_SCRATCH = 2 << 30
 
 
 def streams(n: int, dim: int) -> bool:
@@ -64,8 +68,8 @@ def _k():
             decode=K._sig("b200_kv8_decode", [C.POINTER(_Cache), vp, vp, vp, i, i, vp, i, vp]),
             plan=K._sig("b200_kv8_attention_plan", [i] * 5 + [C.POINTER(i)]),
             attn=K._sig("b200_kv8_attention", [C.POINTER(_Attn)] + [vp] * 5),
-            scratch=K._sig("b200_kv8_prompt_scratch", [i] * 6),
-            prompt=K._sig("b200_kv8_prompt", [C.POINTER(_Cache)] + [vp] * 4 + [i] * 3 + [C.c_float, vp, vp]),
+            scratch=K._sig("b200_kv8_prompt_scratch", [i] * 6 + [ll]),
+            prompt=K._sig("b200_kv8_prompt", [C.POINTER(_Cache)] + [vp] * 4 + [i] * 3 + [C.c_float, ll, vp, vp]),
         )
         _fns.scratch.restype = C.c_longlong
     return _fns
@@ -296,7 +300,9 @@ def _attention_call(cache, q, lens, scale, max_len):
         return lambda cache, q, lens: ref.kv8_attention(q, cache, lens, scale, most)
     group = H // cache.kv_heads
     if not streams(n, D) and scale > 0:
-        return _prompt_call(cache, q, scale, most)
+        call = _prompt_call(cache, q, scale, most)
+        if call is not None:
+            return call
     ok = _aligned(q)
     f, c, device = _k(), cache._c, cache.device
     plan = (C.c_int * 5)()
@@ -329,19 +335,21 @@ def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optio
     """Causal attention of each sequence's n newest tokens: ``q`` [B, n, heads, dim] (bf16), the last one sees the first ``lens[b]`` positions
     of the cache, the one before it one fewer, and so on; one that sees nothing gets zeros.  Returns bf16 [B, n, heads, dim].
     ``scale``: factor of the scores, dim ** -0.5 by default.  ``max_len``: no length is larger (longer ones are cut); the capacity by
-    default.  A smaller bound makes short calls cheaper."""
+    default.  A smaller bound makes short calls cheaper, and those of many tokens take scratch memory for as many keys, at most ``PROMPT_SCRATCH``
+    bytes at a time."""
     if scale is not None:
         scale = float(scale)
     return cache._call((_kind(q), _kind(lens), scale, max_len), _attention_call, q, lens, scale, max_len)(cache, q, lens)
 
 
 def _prompt_call(cache, q, scale, most):
-    """Many query rows per key: the codes become bf16 rows once (exactly), and the prompt attention on the tensor cores reads those."""
+    """Many query rows per key: the codes become bf16 rows once (exactly), and the prompt attention on the tensor cores reads those, a group of
+    sequences and key heads at a time.  None: more tokens than that attention takes."""
     B, n, H, D = q.shape
-    f, device, c, empty_like = _k(), cache.device, C.byref(cache._c), torch.empty_like
-    nbytes = _guarded(device, lambda: f.scratch(B, cache.kv_heads, H, D, n, most))
+    f, device, c, empty_like, limit = _k(), cache.device, C.byref(cache._c), torch.empty_like, PROMPT_SCRATCH
+    nbytes = _guarded(device, lambda: f.scratch(B, cache.kv_heads, H, D, n, most, limit))
     if not nbytes:
-        raise ValueError(f"{B} sequences of {n} tokens and {most} keys are too many for one call")
+        return None
     like, mem_like = (torch.empty(1, dtype=t, device=device).expand(s) for t, s in ((BF16, q.shape), (torch.uint8, (nbytes,))))
     err, contiguous, layout = f.K.err_word(device).data_ptr(), q.is_contiguous(), torch.contiguous_format
 
@@ -350,10 +358,10 @@ def _prompt_call(cache, q, scale, most):
             q = _copy(q)
         out, mem = empty_like(like, memory_format=layout), empty_like(mem_like, memory_format=layout)
         if device.index == _device():
-            f.check(f.prompt(c, q.data_ptr(), lens.data_ptr(), out.data_ptr(), mem.data_ptr(), H, n, most, scale, err, f.stream()), "kv8_prompt")
+            f.check(f.prompt(c, q.data_ptr(), lens.data_ptr(), out.data_ptr(), mem.data_ptr(), H, n, most, scale, limit, err, f.stream()), "kv8_prompt")
         else:
             with torch.cuda.device(device):
-                f.check(f.prompt(c, q.data_ptr(), lens.data_ptr(), out.data_ptr(), mem.data_ptr(), H, n, most, scale, err, f.stream()), "kv8_prompt")
+                f.check(f.prompt(c, q.data_ptr(), lens.data_ptr(), out.data_ptr(), mem.data_ptr(), H, n, most, scale, limit, err, f.stream()), "kv8_prompt")
         return out
 
     return run

@@ -556,3 +556,97 @@ def test_offsets_beyond_two_gigabytes():
         big = (tail[0, h].abs() @ q[0, 0, h].double().abs()).max()
         # the sum of 9.4 million weights of zero scores adds fp32 roundings of partial sums: 2^-24 per addition of a lane, at most 2^-9 in all
         assert ((out[0, 0, h] - want).abs() <= tolerance(want, mag, big, D, F16_HALF + 2.0 ** -9)).all()
+
+
+# ------------------------------------------------------------------------------------------
+# scratch memory of the prompt path
+# ------------------------------------------------------------------------------------------
+def run_in_groups(monkeypatch, limit, B, n, H, Hkv, D, block, cap, lens, device="cuda"):
+    monkeypatch.setattr(kv8, "PROMPT_SCRATCH", limit)
+    cache = filled(B, Hkv, cap, D, block, device, seed=8)
+    q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16)
+    for b in range(B):
+        cache.k.view(torch.uint8)[b, :, lens[b]:] = 0x7F
+        cache.v.view(torch.uint8)[b, :, lens[b]:] = 0xFF
+    out = kv8.attention(q.to(device), cache, i32(lens, device)).double().cpu()
+    k, v = (torch.nan_to_num(values(cache, w)) for w in "kv")
+    want, mag, big = attend(q.double(), k, v, lens, D ** -0.5)
+    tol = tolerance(want, mag, big, D, BF16_HALF)
+    assert ((out - want).abs() <= tol).all(), ((out - want).abs() / tol).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [1, 400_000, 2_000_000])     # a key head of a sequence at a time, a few of them, whole sequences
+@pytest.mark.parametrize("B,n,H,Hkv,D,block,cap,lens", [
+    (3, 100, 6, 6, 96, 16, 304, [300, 99, 0]),
+    (5, 65, 6, 3, 128, 32, 352, [345, 66, 1, 352, 130]),
+    (2, 270, 4, 2, 32, 32, 320, [320, 13]),
+])
+def test_long_attention_in_groups(monkeypatch, limit, B, n, H, Hkv, D, block, cap, lens):
+    """Sequences and key heads answered one group after the other through the same scratch memory, the last group a smaller one."""
+    run_in_groups(monkeypatch, limit, B, n, H, Hkv, D, block, cap, lens)
+
+
+@pytest.mark.gpu
+def test_long_attention_in_groups_nan_reaches_only_those_who_see_it(monkeypatch):
+    monkeypatch.setattr(kv8, "PROMPT_SCRATCH", 1)
+    test_long_attention_nan_reaches_only_those_who_see_it("cuda")
+
+
+def test_prompt_scratch_is_bounded():
+    """Whatever the sizes are, up to what one key head of one sequence takes."""
+    f = kv8._k()
+    for B, Hkv, H, D, n, most in [(64, 8, 32, 128, 64, 32768), (16, 55, 55, 96, 300, 65536), (1, 8, 32, 128, 1500, 8192), (16400, 1, 1, 128, 49, 64),
+                                  (65535, 2, 4, 64, 100, 128), (4, 3, 3, 32, 5000, 1 << 20), (1, 1, 16, 128, 64, 1 << 21), (40000, 1, 1, 128, 50, 1 << 17)]:
+        got = f.scratch(B, Hkv, H, D, n, most, kv8.PROMPT_SCRATCH)
+        least = 2 * ((most + 127) // 128 * 128) * D * 2
+        assert 0 < got <= max(kv8.PROMPT_SCRATCH, least + (64 << 20)), (B, Hkv, n, most, got)
+    assert f.scratch(1, 1, 1, 128, 1 << 23, 1 << 23, kv8.PROMPT_SCRATCH) == 0         # more query tiles than a grid holds: streamed
+
+
+@pytest.mark.gpu
+def test_scratch_of_long_attention_follows_no_capacity():
+    B, n, H, Hkv, D, cap = 64, 64, 8, 8, 128, 16384
+    cache = KV8Cache.empty(B, Hkv, cap, D, "cuda")
+    k = torch.randn(B, 200, Hkv, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    kv8.append(cache, k, k, i32([0] * B, "cuda"))
+    q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    lens = i32([200 - b for b in range(B)], "cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = kv8.attention(q, cache, lens)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 1.1 * kv8.PROMPT_SCRATCH
+    for b in (0, 31, 63):
+        part = KV8Cache(*(t[b:b + 1, :, :256 if t.dim() == 4 else 8].contiguous() for t in (cache.k, cache.v, cache.k_exp, cache.v_exp)))
+        want, mag, big = attend(q[b:b + 1].double().cpu(), values(part, "k"), values(part, "v"), [200 - b], D ** -0.5)
+        assert ((out[b:b + 1].double().cpu() - want).abs() <= tolerance(want, mag, big, D, BF16_HALF)).all()
+
+
+@pytest.mark.gpu
+def test_long_attention_of_more_sequences_than_a_grid_of_tiles_holds():
+    B, n, D, cap = 16400, 49, 128, 64
+    assert not kv8.streams(n, D)
+    cache = KV8Cache.empty(B, 1, cap, D, "cuda")
+    k, v = (torch.randn(B, cap, 1, D, device="cuda", generator=torch.Generator("cuda").manual_seed(s)).to(torch.bfloat16) for s in (1, 2))
+    kv8.append(cache, k, v, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    q = torch.randn(B, n, 1, D, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(torch.bfloat16)
+    lens = (torch.arange(B, device="cuda") % (cap + 1)).int()
+    out = kv8.attention(q, cache, lens)
+    for b in (0, 1, 63, 8200, 16383, 16384, 16399):
+        part = KV8Cache(*(t[b:b + 1].contiguous() for t in (cache.k, cache.v, cache.k_exp, cache.v_exp)))
+        want, mag, big = attend(q[b:b + 1].double().cpu(), values(part, "k"), values(part, "v"), [b % (cap + 1)], D ** -0.5)
+        assert ((out[b:b + 1].double().cpu() - want).abs() <= tolerance(want, mag, big, D, BF16_HALF)).all()
+
+
+@pytest.mark.gpu
+def test_what_the_tiles_do_not_take_is_streamed(monkeypatch):
+    monkeypatch.setattr(kv8, "_prompt_call", lambda *a: None)
+    B, n, H, Hkv, D, block, cap = 2, 100, 4, 2, 128, 32, 352
+    assert not kv8.streams(n, D)
+    cache = filled(B, Hkv, cap, D, block, "cuda", seed=8)
+    q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(7)).to(torch.bfloat16)
+    out = kv8.attention(q.cuda(), cache, i32([345, 66], "cuda")).double().cpu()
+    want, mag, big = attend(q.double(), values(cache, "k"), values(cache, "v"), [345, 66], D ** -0.5)
+    assert ((out - want).abs() <= tolerance(want, mag, big, D, F16_HALF)).all()
