@@ -10,7 +10,8 @@ again forgets what lies behind it in the block.  Infinities are stored as the bl
 
 Sequences are described by int32 tensors on the cache's device and never read by the host: positions outside the cache are left out by
 the kernels (nothing is written) and recorded in the device status word (``cuda.check_device_status``), lengths are cut to the capacity.
-Calls run on the current stream and allocate through PyTorch's allocator.  They belong to decoding: none has a gradient."""
+Calls run on the current stream and allocate through PyTorch's allocator.  They belong to decoding: their results carry no
+gradient, whatever requires one."""
 from __future__ import annotations
 
 import ctypes as C

@@ -365,6 +365,7 @@ def _kv8_put(codes, exps, x, start: int, block: int) -> None:
         exps[:, lo // block] = e.to(torch.int8)
 
 
+@torch.no_grad()
 def kv8_append(cache, k, v, start, counts=None) -> None:
     """Positions start[b] .. of the cache become the first counts[b] tokens of k, v [B, n, Hkv, D]; a sequence that does not fit is left out."""
     n = k.shape[1]
@@ -376,6 +377,7 @@ def kv8_append(cache, k, v, start, counts=None) -> None:
         _kv8_put(cache.v[b], cache.v_exp[b], v[b, :c].float(), at, cache.block)
 
 
+@torch.no_grad()
 def kv8_rope_append(cache, qkv, cos, sin, pos, heads, bias=None, clear=False) -> torch.Tensor:
     """Bias, rotation of neighbouring pairs and cache append of one new token per sequence, in fp32; q rounded once."""
     B, D, Hkv = cache.batch, cache.dim, cache.kv_heads
@@ -396,6 +398,7 @@ def kv8_rope_append(cache, qkv, cos, sin, pos, heads, bias=None, clear=False) ->
     return q
 
 
+@torch.no_grad()
 def kv8_attention(q, cache, lens, scale: float, max_len: int) -> torch.Tensor:
     """Query i of n sees the first lens[b] - (n - 1 - i) positions of the cache; without any its output is zero."""
     B, n, H, D = q.shape

@@ -650,3 +650,23 @@ def test_what_the_tiles_do_not_take_is_streamed(monkeypatch):
     out = kv8.attention(q.cuda(), cache, i32([345, 66], "cuda")).double().cpu()
     want, mag, big = attend(q.double(), values(cache, "k"), values(cache, "v"), [345, 66], D ** -0.5)
     assert ((out - want).abs() <= tolerance(want, mag, big, D, F16_HALF)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [1, 60])
+def test_results_carry_no_gradient(device, n):
+    """On either device, whatever requires one; an accumulator that requires one may be cleared."""
+    B, H, Hkv, D = 2, 4, 2, 128
+    cache = filled(B, Hkv, 96, D, 32, device)
+    q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(device).requires_grad_()
+    assert not kv8.attention(q, cache, i32([90, 70], device)).requires_grad
+    assert not kv8.attention(q[:, :0], cache, i32([90, 70], device)).requires_grad
+    cos, sin = tables(96, D, device)
+    qkv = torch.randn(B, (H + 2 * Hkv) * D, device=device, requires_grad=True)
+    bias = torch.randn((H + Hkv) * D, device=device, requires_grad=True)
+    assert not kv8.rope_append(cache, qkv, cos, sin, i32([3, 4], device), H, bias=bias).requires_grad
+    assert not kv8.rope_append(cache, qkv, cos, sin, i32([5, 6], device), H, bias=bias, clear=True).requires_grad
+    assert not qkv.detach().any()
+    k = torch.randn(B, 3, Hkv, D, device=device).to(torch.bfloat16).requires_grad_()
+    kv8.append(cache, k, k, i32([7, 8], device))
+    assert not any(t.requires_grad for t in (cache.k, cache.v, cache.k_exp, cache.v_exp, *cache.decoded()))
