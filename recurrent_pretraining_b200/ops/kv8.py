@@ -252,7 +252,8 @@ def _rope_call(cache, qkv, cos, sin, pos, heads, bias, clear):
     _index(pos, cache, "pos")
     ld = 0 if B == 1 else qkv.stride(0)
     err = _k().K.err_word(cache.device).data_ptr() if cache.k.is_cuda else 0
-    return torch.empty(B, heads, D, dtype=BF16, device=cache.device), C.byref(cache._c), ld, int(qkv.dtype == F32), not (ld * qkv.element_size() & 15), err
+    like = torch.empty(1, dtype=BF16, device=cache.device).expand(B, heads, D)        # a template of one element: an engine has many caches
+    return like, C.byref(cache._c), ld, int(qkv.dtype == F32), not (ld * qkv.element_size() & 15), err
 
 
 def rope_append(cache: KV8Cache, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, heads: int,
@@ -272,7 +273,7 @@ def rope_append(cache: KV8Cache, qkv: torch.Tensor, cos: torch.Tensor, sin: torc
         return rope_append(cache, _copy(qkv), cos, sin, pos, heads, bias)
     if (cp | sp) & 15:
         return rope_append(cache, qkv, cos.clone(), sin.clone(), pos, heads, bias, clear)
-    f, q, bp = _fns, torch.empty_like(like), 0 if bias is None else bias.data_ptr()
+    f, q, bp = _fns, torch.empty_like(like, memory_format=torch.contiguous_format), 0 if bias is None else bias.data_ptr()
     if cache.device.index == _device():
         f.check(f.rope(c, x, ld, f32, clear, bp, cp, sp, pos.data_ptr(), q.data_ptr(), heads, err, f.stream()), "kv8_rope_append")
     else:

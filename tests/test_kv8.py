@@ -670,3 +670,16 @@ def test_results_carry_no_gradient(device, n):
     k = torch.randn(B, 3, Hkv, D, device=device).to(torch.bfloat16).requires_grad_()
     kv8.append(cache, k, k, i32([7, 8], device))
     assert not any(t.requires_grad for t in (cache.k, cache.v, cache.k_exp, cache.v_exp, *cache.decoded()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_what_a_cache_remembers_of_its_calls_is_small(device):
+    """Plans and templates, no buffers of a call's size: an engine keeps a cache per layer and recurrence."""
+    B, H, Hkv, D = 8, 16, 4, 64
+    cache = filled(B, Hkv, 96, D, 32, device)
+    cos, sin = tables(96, D, device)
+    q = kv8.rope_append(cache, torch.randn(B, (H + 2 * Hkv) * D, device=device), cos, sin, i32([3] * B, device), H)
+    kv8.attention(q[:, None], cache, i32([4] * B, device))
+    kept = [x for call in cache._calls.values() if isinstance(call, tuple) for x in call if torch.is_tensor(x)]
+    assert sum(t.untyped_storage().nbytes() for t in kept) <= 64
+    assert q.shape == (B, H, D) and q.is_contiguous()
