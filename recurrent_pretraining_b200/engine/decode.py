@@ -105,8 +105,7 @@ class StaticRecurrentKV8Cache(StaticRecurrentKVCache):
         kv8.append(layer, k, v, torch.full((k.shape[0],), end - n, dtype=torch.int32, device=k.device))
         if end == n:
             return k, v
-        k, v = layer.decoded()
-        return k[:, :end], v[:, :end]
+        return layer.decoded(end)
 
     def get_memory_usage(self) -> float:
         return sum(t.numel() for t in (self.k, self.v, self.k_exp, self.v_exp)) / 2**20

@@ -142,14 +142,18 @@ class KV8Cache:
         codes = [torch.zeros(batch, kv_heads, n * block, dim, dtype=torch.uint8, device=device).view(E4M3) for _ in range(2)]
         return cls(*codes, *(torch.full((batch, kv_heads, n), ref.KV8_EMIN, dtype=torch.int8, device=device) for _ in range(2)))
 
-    def decoded(self) -> tuple:
-        """Keys and values of all positions as bf16 [B, capacity, kv_heads, dim] (exact)."""
+    def decoded(self, length: Optional[int] = None) -> tuple:
+        """Keys and values of the first ``length`` positions (all by default) as bf16 [B, length, kv_heads, dim] (exact)."""
+        n = self.capacity if length is None else int(length)
+        if not 0 < n <= self.capacity:
+            raise ValueError(f"length lies in 1 .. {self.capacity}")
         if not self.k.is_cuda:
-            return tuple(ref.kv8_decode(c, e).transpose(1, 2).to(BF16) for c, e in ((self.k, self.k_exp), (self.v, self.v_exp)))
-        k, v = (torch.empty(self.batch, self.capacity, self.kv_heads, self.dim, dtype=BF16, device=self.device) for _ in range(2))
+            blocks = (n + self.block - 1) // self.block
+            return tuple(ref.kv8_decode(c[:, :, :blocks * self.block], e[:, :, :blocks])[:, :, :n].transpose(1, 2).to(BF16, memory_format=torch.contiguous_format)
+                         for c, e in ((self.k, self.k_exp), (self.v, self.v_exp)))
+        k, v = (torch.empty(self.batch, n, self.kv_heads, self.dim, dtype=BF16, device=self.device) for _ in range(2))
         f = _k()
-        _guarded(self.device, lambda: f.K._check(f.decode(C.byref(self._c), 0, k.data_ptr(), v.data_ptr(), self.capacity, self.capacity, 0, 0, f.K._stream()),
-                                                 "kv8_decode"))
+        _guarded(self.device, lambda: f.K._check(f.decode(C.byref(self._c), 0, k.data_ptr(), v.data_ptr(), n, n, 0, 0, f.K._stream()), "kv8_decode"))
         return k, v
 
     def _call(self, key: tuple, make, *args):

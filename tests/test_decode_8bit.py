@@ -225,3 +225,16 @@ def test_rows_without_a_finite_logit_are_reported(model, new):
             model.lm_head.weight.copy_(keep)
     tokens, stats = eng.generate(ids, new, init_scale=0.0, sampling=hot)
     assert stats["device_status"] == 0 and (tokens >= 0).all()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_a_second_chunk_decodes_what_it_reads(device):
+    """The codes of the positions so far, not of the capacity."""
+    from recurrent_pretraining_b200.engine.decode import StaticRecurrentKV8Cache
+
+    cache = StaticRecurrentKV8Cache(1, 2, 5000, 5, 96, device, 1, 0, 0)
+    k = torch.randn(2, 70, 5, 96, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).to(device)
+    cache.update(k[:, :33], k[:, :33], 0)
+    for got in cache.update(k[:, 33:], k[:, 33:], 0):
+        assert got.shape == (2, 70, 5, 96) and got.untyped_storage().nbytes() == k.untyped_storage().nbytes()
+        assert ((got.float() - k.float()).abs() <= 2.0 ** -3 * k.float().abs() + 2.0 ** -8).all()          # two roundings to e4m3 at most

@@ -683,3 +683,17 @@ def test_what_a_cache_remembers_of_its_calls_is_small(device):
     kept = [x for call in cache._calls.values() if isinstance(call, tuple) for x in call if torch.is_tensor(x)]
     assert sum(t.untyped_storage().nbytes() for t in kept) <= 64
     assert q.shape == (B, H, D) and q.is_contiguous()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_decoded_positions(device):
+    """Keys and values of the first positions only: memory for those, whatever the capacity is."""
+    cache = filled(2, 3, 320, 96, 32, device)
+    whole = cache.decoded()
+    for length in (1, 31, 130, 320):
+        for got, all_, which in zip(cache.decoded(length), whole, "kv"):
+            assert got.shape == (2, length, 3, 96) and got.untyped_storage().nbytes() == 2 * 2 * length * 3 * 96
+            assert torch.equal(got, all_[:, :length]) and torch.equal(got.double().cpu(), values(cache, which)[:, :, :length].transpose(1, 2))
+    for bad in (0, -1, 321):
+        with pytest.raises(ValueError):
+            cache.decoded(bad)
