@@ -581,39 +581,59 @@ sample_kernel(const SampleParams p) {
 
 using namespace b200;
 
+// CTAs per row: as many as the machine holds at a time (two per SM) and slices of more than 1024 elements allow; at most 40960 to a slice.  For few rows
+// a cluster beyond the portable size, on a device that schedules one (`wide`).
+B200_API int b200_sample_ctas(int B, int V, int sms, int wide) {
+  int C = 1;
+  while (C < 8 && ((V + C - 1) / C > 40960 || (static_cast<long long>(B) * C <= sms && (V + C - 1) / C > 1024))) C *= 2;
+  if (C == 8 && wide && B <= 4 && (V + C - 1) / C > 2048) C = 16;
+  return C;
+}
+static int sample_per(int V, int C) { return ((V + C - 1) / C + SP_THREADS - 1) / SP_THREADS * SP_THREADS; }
+static int sample_smem(int per) { return (per + per / 32) * 4; }
+
 // logits: [B, V] (pitch ld elements), bf16 or fp32; uniform: [B]; per-row tensors may be null (then t, k, p, m hold); out: int64 [B].
 B200_API int b200_sample(const SampleParams* a, int B, int is_bf16, void* stream) {
   SampleParams p = *a;
-  if (B <= 0 || p.V <= 0 || p.ld < p.V || !p.logits || !p.uniform || !p.out) return -1;
-  int C = 1;
-  // as many CTAs per row as the machine holds at a time (two per SM) and slices of more than 1024 elements allow; at most 40960 to a slice
-  while (C < 8 && ((p.V + C - 1) / C > 40960 || (static_cast<long long>(B) * 2 * C <= 296 && (p.V + C - 1) / C > 1024))) C *= 2;
-  if (C == 8 && B <= 4 && (p.V + C - 1) / C > 2048) C = 16;        // beyond the portable size, for few rows
-  p.per = ((p.V + C - 1) / C + SP_THREADS - 1) / SP_THREADS * SP_THREADS;
-  const int smem = (p.per + p.per / 32) * 4;
-  if (smem > SP_MAX_SMEM || static_cast<long long>(B) * C > (1ll << 31) - 1) return -2;
+  if (B <= 0 || p.V <= 0 || p.V > 8 * 40960 || p.ld < p.V || !p.logits || !p.uniform || !p.out) return -1;
   auto kern = is_bf16 ? sample_kernel<__nv_bfloat16> : sample_kernel<float>;
   int dev = 0;
-  static bool configured[64][2] = {};               // the same attributes for every call: threads may set them twice
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
-  if (!configured[dev][is_bf16 != 0]) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_MAX_SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return -4;
-    configured[dev][is_bf16 != 0] = true;
-  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(B * C));
-  cfg.blockDim = dim3(SP_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.x = 16;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.blockDim = dim3(SP_THREADS);
   cfg.attrs = at;
+  struct Device { int sms, wide; };
+  static Device known[64][2] = {};                  // the same for every call: threads may find them twice
+  Device& d = known[dev][is_bf16 != 0];
+  if (!d.sms) {
+    Device x = {};
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_MAX_SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaDeviceGetAttribute(&x.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return -4;
+    cfg.gridDim = dim3(16);
+    cfg.dynamicSmemBytes = sample_smem(sample_per(8 * 40960, 16));              // of the longest rows
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess) cudaGetLastError();       // none, then
+    x.wide = clusters > 0;
+    d.wide = x.wide;
+    d.sms = x.sms;
+  }
+  const int C = b200_sample_ctas(B, p.V, d.sms, d.wide);
+  p.per = sample_per(p.V, C);
+  const int smem = sample_smem(p.per);
+  if (smem > SP_MAX_SMEM || static_cast<long long>(B) * C > (1ll << 31) - 1) return -2;
+  cfg.gridDim = dim3(static_cast<unsigned>(B * C));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  at[0].val.clusterDim.x = C;
   cfg.numAttrs = g_b200_pdl ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? 0 : -10;
 }

@@ -248,3 +248,20 @@ def test_a_min_p_of_one_keeps_the_largest_alone(device):
     x[1, [10, 2000, 2500]] = torch.tensor([4.0, 4.0, 3.9999998])
     for u, want in ((0.0, [2000, 10]), (0.4, [2000, 10]), (0.9, [2000, 2000])):
         assert sample_tokens(x.to(device), torch.full((2,), u, device=device), min_p=1.0).tolist() == want
+
+
+def test_ctas_of_a_row_follow_the_device():
+    import ctypes as C
+
+    from recurrent_pretraining_b200.ops import cuda as K
+
+    ctas = K._sig("b200_sample_ctas", [C.c_int] * 4)
+    for sms in (148, 74, 1):
+        for wide in (0, 1):
+            for B in (1, 4, 5, 18, 64, 5000):
+                for V in (1, 1024, 1025, 32003, 65536, MAX_VOCAB):
+                    c = ctas(B, V, sms, wide)
+                    assert c in (1, 2, 4, 8, 16) and (c < 16 or (wide and B <= 4)) and -(-V // c) <= 40960
+                    assert c == 1 or -(-V // (c // 2)) > 1024                          # no slices that are not worth a CTA
+                    assert B * c <= 2 * sms or c in (1, 16) or -(-V // (c // 2)) > 40960
+    assert [ctas(b, 65536, 148, 1) for b in (1, 4, 5, 18, 64, 200)] == [16, 16, 8, 8, 4, 2]
