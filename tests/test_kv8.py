@@ -697,3 +697,19 @@ def test_decoded_positions(device):
     for bad in (0, -1, 321):
         with pytest.raises(ValueError):
             cache.decoded(bad)
+
+
+@pytest.mark.gpu
+def test_a_sequence_alone_and_in_a_batch():
+    """Shares are cut from the lengths of all sequences, so the order of a sum follows the batch; the result stays within its tolerance."""
+    B, n, H, Hkv, D, cap = 6, 2, 6, 3, 96, 1504
+    cache = filled(B, Hkv, cap, D, 32, "cuda")
+    q = torch.randn(B, n, H, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    lens = [1500, 3, 900, 0, 1024, 77]
+    whole = kv8.attention(q.cuda(), cache, i32(lens, "cuda")).double().cpu()
+    for b in range(B):
+        alone = KV8Cache(*(t[b:b + 1] for t in (cache.k, cache.v, cache.k_exp, cache.v_exp)))
+        one = kv8.attention(q[b:b + 1].cuda(), alone, i32(lens[b:b + 1], "cuda")).double().cpu()
+        want, mag, big = attend(q[b:b + 1].double(), values(alone, "k"), values(alone, "v"), lens[b:b + 1], D ** -0.5)
+        tol = tolerance(want, mag, big, D, F16_HALF)
+        assert ((one - want).abs() <= tol).all() and ((whole[b:b + 1] - want).abs() <= tol).all()
