@@ -238,3 +238,77 @@ def test_a_second_chunk_decodes_what_it_reads(device):
     for got in cache.update(k[:, 33:], k[:, 33:], 0):
         assert got.shape == (2, 70, 5, 96) and got.untyped_storage().nbytes() == k.untyped_storage().nbytes()
         assert ((got.float() - k.float()).abs() <= 2.0 ** -3 * k.float().abs() + 2.0 ** -8).all()          # two roundings to e4m3 at most
+
+
+@gpu
+@pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("use_graphs", [False, True])
+def test_every_sampled_token_is_drawn_from_the_generators_numbers(model, use_graphs, kv_dtype):
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+    from recurrent_pretraining_b200.models.sampling import SamplingOptions
+
+    ids = torch.randint(0, 4000, (3, 20), device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    eng = DecodeEngine(model, max_batch=3, max_len=64, num_steps=4, use_graphs=use_graphs, kv_dtype=kv_dtype)
+    for seed in (3, 4):
+        toks, _ = eng.generate(ids, 12, init_scale=0.0, sampling=SamplingOptions(**FLAT), generator=torch.Generator("cuda").manual_seed(seed))
+        assert torch.equal(toks[:, 20:], places(torch.Generator("cuda").manual_seed(seed), 3, eng.V, 12))
+
+
+def test_numbers_take_their_place_where_weights_are_equal():
+    from recurrent_pretraining_b200.ops.sampling import sample_tokens
+
+    u = torch.rand(500, generator=torch.Generator().manual_seed(1))
+    x = torch.randn(500, 4096, generator=torch.Generator().manual_seed(2))
+    assert torch.equal(sample_tokens(x, u, temperature=1e30), (u.double() * 4096).floor().long())
+
+
+@gpu
+@pytest.mark.parametrize("strategy", ["full", "full-compress-s4", "full-compress-s1"])
+def test_slots_of_the_8bit_cache_hold_what_the_bf16_cache_holds(model, strategy):
+    """Both engines over the same tokens.  A prompt's slots differ by one rounding to e4m3 of equal values; those of later tokens, whose hidden states saw
+    rounded keys and values (3 % of noise each), by far less than a wrong exponent (a factor of two) would make of them."""
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+
+    B, P, steps = 2, 41, 9
+    ids = torch.randint(0, 4000, (B, P + steps), device="cuda", generator=torch.Generator("cuda").manual_seed(8))
+    half, fp8 = (DecodeEngine(model, max_batch=B, max_len=64, num_steps=4, cache_lookup_strategy=strategy, kv_dtype=t) for t in ("bf16", "fp8"))
+
+    def slots():
+        for s in range(half.cache.n_slots):
+            yield from zip((half.cache.k[s].float(), half.cache.v[s].float()), (t[:, :half.Lmax].float() for t in fp8.cache.layers[s].decoded()),
+                           (fp8.cache.k_exp[s], fp8.cache.v_exp[s]))
+
+    with torch.no_grad():
+        for eng in (half, fp8):
+            eng.prefill(ids[:, :P], init_scale=0.0)
+        for want, got, exps in slots():
+            step = torch.exp2(exps.float()).repeat_interleave(32, -1)[:, :, :half.Lmax].transpose(1, 2)[..., None]         # of a code below 2^-6
+            tol = (2.0 ** -4 + 2.0 ** -8) * want.abs() + 2.0 ** -10 * step
+            assert ((got - want).abs() <= tol)[:, :P].all()
+        for i in range(steps):
+            logits = []
+            for eng in (half, fp8):
+                eng.tok.copy_(ids[:, P + i])
+                eng._fresh_state(0.0)
+                eng._token_fixed(4, False)
+                eng.pos.add_(1)
+                eng.lens.add_(1)
+                logits.append(eng.logits.float())
+            assert ((logits[0] - logits[1]).abs() <= 0.15 + 0.25 * logits[0].std(-1, keepdim=True)).all()
+        for want, got, _ in slots():
+            for at in range(P, P + steps):
+                assert (got[:, at] - want[:, at]).norm() <= 0.15 * want[:, at].norm()
+            assert (got[:, :P] - want[:, :P]).norm() <= 0.15 * want[:, :P].norm()
+
+
+@gpu
+@pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
+def test_kl_decoding_that_never_exits_is_greedy_decoding(model, kv_dtype):
+    """A threshold that no divergence is below: every token takes all recurrences and is (nearly) the model's largest logit."""
+    from recurrent_pretraining_b200.engine.decode import DecodeEngine
+
+    ids = torch.randint(0, 4000, (2, 16), device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    eng = DecodeEngine(model, max_batch=2, max_len=48, num_steps=4, kv_dtype=kv_dtype)
+    toks, stats = eng.generate(ids, 9, criterion="kl", exit_threshold=-1.0, max_steps=4, init_scale=0.0)
+    assert stats["device_status"] == 0 and stats["steps"] == [[4, 4]] * 8
+    assert nearly_largest(model, toks, 16)
