@@ -26,12 +26,12 @@ struct Kv8Cache {
   int B, Hkv, cap, D, log2_block;
 };
 
-// Threads for a block of so many values, 24 to 96 values each.  4 x 1024 tokens of 5280 channels, 20 us of copying: 20.1 to 22.3 us with every block and
-// dim but 16 x 32 (25.1).  2048 values take 25.5 with 128 threads, 23.7 with 64, 21.8 with a warp; 16384 take 26.3 with 128 threads, 20.7 with 256.
+// Threads for a block of so many values, 16 to 96 values each.  4 x 1024 tokens of 5280 channels (the one shape that the borders were measured at; a
+// call of few tokens is bound by its launch), 20 us of copying: 20.1 to 22.3 us with every block and dim but 16 x 32 (25.1).  2048 values take 25.5 with 128 threads, 23.7 with 64, 21.8 with a warp; 16384 take 26.3 with 128 threads, 20.7 with 256.
 __host__ __device__ constexpr int kv8_group(int values) { return values <= 2048 ? 32 : values <= 12288 ? 128 : 256; }
 __host__ __device__ constexpr int kv8_threads(int G) { return G > 32 ? G : 128; }
 
-// grid (2 x most touched blocks / (128 / G), Hkv, B), 128 threads, G of them (a warp or the CTA) per block of BLK tokens.  The block's new tokens
+// grid (2 x most touched blocks / (threads / G), Hkv, B), kv8_threads(G) threads, G of them (a warp or the CTA) per block of BLK tokens.  The block's new tokens
 // stay in registers (NV vectors of eight values per thread) between the maximum and the encoding: one pass over the input.  D and BLK
 // are known to the compiler: a division per vector would take longer than the vector.
 template <int D, int BLK, int G>

@@ -6,8 +6,8 @@
 // D + D bytes per key, and everything else has to hide behind it.  A warp takes 32 keys at a time through a ring of its own (cp.async, no
 // barriers between warps) and forms both products transposed, S^T = K Q^T and O^T = V^T P^T, with mma.sync m16n8k16 on f16: the
 // keys (the channels of V) fill the 16 rows, eight query rows the columns.  f16 holds every e4m3 value exactly, and each code is
-// widened once.  Transposing matrix loads of bytes turn V.  (mma.sync on 8-bit types is emulated on this machine: a step of 32 keys took 757
-// instructions with it, 410 with f16.  tcgen05 takes codes as they are, but then q and the weights
+// widened once.  Transposing matrix loads of bytes turn V.  (mma.sync on 8-bit types was tried first and
+// took more instructions per step than widening.  tcgen05 takes codes as they are, but then q and the weights
 // have to be split into 8-bit parts, four products each, and a tile's maximum and weights go through barriers of the whole CTA.)
 //
 // q enters as f16 under a power of two per row, which keeps bf16's eight bits down to 2^-28 of the row's largest.  Weights enter as f16

@@ -14,8 +14,9 @@
 //
 // A row is bound by the latency of its stages: 17.5 us for 65536 fp32 logits with top-p 0.95 on 16 CTAs (read 1.4, maximum 1.4, histogram 2.6, its
 // exchange and border 4.4, candidates 2, ranking 2.5, kept list 1.5, token 1.7), where the bytes would take 0.04.  A batch of 64 such rows with settings of
-// their own (4 CTAs each, two per SM) takes 41.5 us: 14 of them are the histogram pass, bound by the instructions that form the weights (atomics 3,
-// the table 1, both measured by leaving them out).
+// their own (4 CTAs each, two per SM) takes 41.3 us: 14 of them are the histogram pass, bound by the instructions that form the weights (atomics 3,
+// the table 1, both measured by leaving them out).  Differences of two logits and their exponents are formed in double precision: either may lie outside
+// fp32, and the products' common rounding, 2^-53 of max / T, stays below a weight's last bit for logits of up to some hundreds of temperatures.
 #include <cooperative_groups.h>
 
 #include <utility>
@@ -29,7 +30,7 @@ constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_BINS = 512, SP_CA
 constexpr int SP_SEG = SP_THREADS / SP_FEW;         // threads that rank a candidate
 constexpr float SP_BINS_PER_OCTAVE = 32.f;
 constexpr int SP_MAX_SMEM = 180 * 1024;             // for the slice
-constexpr int SP_ONE = 44;                          // a weight of 1 is 2^44; 2^18 of them fit the sums
+constexpr int SP_ONE = 44;                          // a weight of 1 is 2^44; 2^20 of them fit the sums (a row has 327680 at most)
 static_assert(SP_BINS == SP_THREADS, "a bin per thread");
 
 struct SampleParams {

@@ -35,7 +35,9 @@ def streams(n: int, dim: int) -> bool:
     bf16 rows by the prompt attention, whose tiles are filled by the tokens of one head.  Microseconds of both ways at 8 sequences of 4096 keys
     and 8 key heads: dim 64, 4 heads per key head: 64 tokens 95 / 124, 128 tokens 176 / 126; dim 128, 1 head: 64 tokens 64 / 70, 128 tokens
     99 / 72; 16 heads: 32 tokens 281 / 446, 64 tokens 537 / 447.  They are equal at about 105 (94), 95 (75), 80 (64) and 62 (52) tokens
-    for dims of 32, 64, 96 and 128 with 4 (16) heads per key head."""
+    for dims of 32, 64, 96 and 128 with 4 (16) heads per key head.  Neither batch nor length enters, so few tiles
+    of long sequences are answered later than they could be: 1 sequence of 65536 keys, 16 key heads of 128, 1 head each: 64 tokens 160 / 357, 128 tokens
+    280 / 355, 256 tokens 516 / 374."""
     return n <= 112 - dim // 2
 
 
@@ -340,6 +342,8 @@ def _attention_call(cache, q, lens, scale, max_len):
 def attention(q: torch.Tensor, cache: KV8Cache, lens: torch.Tensor, scale: Optional[float] = None, max_len: Optional[int] = None) -> torch.Tensor:
     """Causal attention of each sequence's n newest tokens: ``q`` [B, n, heads, dim] (bf16), the last one sees the first ``lens[b]`` positions
     of the cache, the one before it one fewer, and so on; one that sees nothing gets zeros.  Returns bf16 [B, n, heads, dim].
+    Scores and sums are fp32; the weights enter their product with V in 11 bits where codes are streamed, in bf16's 8 where ``streams`` says no (long
+    prompts: 0.0022 off the result in 64 bits, of which rounding the output is 0.0017).
     ``scale``: factor of the scores, dim ** -0.5 by default.  ``max_len``: no length is larger (longer ones are cut); the capacity by
     default.  A smaller bound makes short calls cheaper, and those of many tokens take scratch memory for as many keys, at most ``PROMPT_SCRATCH``
     bytes at a time."""
